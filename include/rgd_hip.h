@@ -308,6 +308,72 @@ int rgd_attn_bwd(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t D,
                  int dtype, int causal, float softmax_scale, int mode, const void* bias_classes,
                  void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Paged key/value cache: new tokens appended with their rotation, and the attention of one new token per
+ * sequence over it.  No counterpart in the reference (it has no cache).
+ *
+ * A cache is (num_pages, H, page_size, D) given as (page, head, slot) strides in an rgd_tensor4 (stride_b = page),
+ * so that token-major and head-major storage are both views of it; keys and values have separate descriptors of the
+ * same sizes.  Position t of sequence b lives in page page_table[b * table_stride + t / page_size], slot t % page_size;
+ * page_table and the length arrays are int32 device memory.  Positions lie in [0, max_pages * page_size), which must
+ * be below 2^31.  A page number outside [0, num_pages) is no page: such a token is not stored, such a key not seen.
+ * fp16 or bf16, D <= 128; any strides, 16-byte accesses where pointers, strides, D and R allow them.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Token t < T of sequence b gets position cache_lens[b] + t.  Tokens with t >= new_lens[b] (new_lens NULL: none) and
+ * tokens whose position lies outside the page table are padding: nothing is stored, their row of qo is zero.  For the others
+ *   qo[b, :, t]       = rot(norm(q[b, :, t]))     key cache slot = rot(norm(k[b, :, t]))     value cache slot = v[b, :, t]
+ * rot as in rgd_rope_qk with the table row of the position (channels < R of positions < q_cutoff / k_cutoff; R even),
+ * norm the LayerNorm over D without affine when layer_norm != 0, else nothing.  R > 0 needs P >= max_pages * page_size.
+ * Cache rows of no new token are left as they were.  cache_lens itself is not changed.  Two tokens of one call must not fall
+ * on the same slot (a page that stands twice in the table; what the slot then holds is undefined).  qo may be q. */
+int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                          const rgd_tensor4* q, const rgd_tensor4* k, const rgd_tensor4* v, const rgd_tensor4* qo,
+                          const rgd_tensor4* k_cache, const rgd_tensor4* v_cache, int64_t num_pages, int64_t page_size,
+                          const int32_t* page_table, int64_t max_pages, int64_t table_stride,
+                          const int32_t* cache_lens, const int32_t* new_lens,
+                          const void* pos_emb, int64_t P, int64_t R, int64_t pe_stride_s, int64_t pe_stride_n,
+                          int pe_dtype, int64_t q_cutoff, int64_t k_cutoff, int layer_norm, float eps,
+                          int dtype, void* stream);
+
+/* o[b, h] = sum_j softmax_j(softmax_scale q[b, h] . k_j + bias_j) v_j over the positions j < seq_lens[b] (the new token's
+ * own key is among them), h reading key head h / (Hq / Hkv).  q and o use stride_b and stride_h.  lse (NULL or fp32 (B, Hq))
+ * receives log sum_j exp of the logits.  A sequence without keys, or with no logit above -inf, gives o = 0 and lse = -inf.
+ * rel_weight (NULL: no bias): bias_j = weight[bucket * w_stride + h] of the range (see rgd_rel_bias_fwd) that holds
+ * j - (seq_lens[b] - 1); starts and buckets are HOST arrays, read during the call.
+ * Statistics and sums are fp32; every result is reproducible bit for bit.  Calls that may overlap in time need separate
+ * workspaces (any contents on entry, 16-byte aligned). */
+size_t rgd_paged_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
+int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_tensor4* q,
+                     const rgd_tensor4* k_cache, const rgd_tensor4* v_cache, int64_t num_pages, int64_t page_size,
+                     const int32_t* page_table, int64_t max_pages, int64_t table_stride, const int32_t* seq_lens,
+                     const void* rel_weight, int64_t w_stride, int64_t num_buckets, int w_dtype,
+                     int64_t n_ranges, const int32_t* starts, const int32_t* buckets,
+                     const rgd_tensor4* o, float* lse, int dtype, float softmax_scale,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Learned relative position bias, an attention bias (1, H, Tq, Tk) from a weight (num_buckets, H).  No counterpart in
+ * the reference (its bias is the caller's).
+ *   bias[h, i, j] = weight[bucket(d) * w_stride + h],  d = j - i - q_offset
+ * Buckets are ranges of d: range k < n_ranges holds starts[k] <= d < starts[k + 1] and has bucket buckets[k]; range 0 holds
+ * everything below starts[1] (starts[0] is not read) and the last one everything from its start on.  Starts ascend and
+ * no bucket has two ranges; starts and buckets are HOST arrays, read during the call; at most 256 ranges and buckets.
+ * ------------------------------------------------------------------------------------------ */
+
+/* bias by (head, row) strides (stride_h, stride_n), any dtype */
+int rgd_rel_bias_fwd(int64_t H, int64_t Tq, int64_t Tk, const void* weight, int64_t w_stride, int64_t num_buckets,
+                     int w_dtype, int64_t n_ranges, const int32_t* starts, const int32_t* buckets, int64_t q_offset,
+                     const rgd_tensor4* bias, int bias_dtype, void* stream);
+
+/* dweight[b * dw_stride + h] = sum of dbias[h, i, j] over the pairs whose d lies in bucket b (0 for a bucket without a range):
+ * fp32 sums in a fixed order, rounded once to the weight's type.  Scratch: any contents on entry, 16-byte aligned. */
+size_t rgd_rel_bias_bwd_workspace(int64_t H, int64_t Tq, int64_t Tk);
+int rgd_rel_bias_bwd(int64_t H, int64_t Tq, int64_t Tk, const rgd_tensor4* dbias, int dbias_dtype,
+                     int64_t n_ranges, const int32_t* starts, const int32_t* buckets, int64_t q_offset,
+                     void* dweight, int64_t dw_stride, int64_t num_buckets, int dw_dtype,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,7 +18,9 @@ Differences from the reference, all deliberate:
     signatures instead of a compiled-kernel handle, so a change of shape, dtype or bias kind after
     the first call can never reuse a stale specialisation.
 """
+import contextlib
 import ctypes
+import functools
 import math
 import os
 
@@ -30,7 +32,7 @@ from ._hip import t3, t4
 __all__ = [
     "flash_attn_func", "triton_rms_func_fn", "triton_fused_rms_func_fn", "triton_fused_ln_func_fn",
     "triton_norm_func_fn", "triton_fused_norm_func_fn", "triton_rope_fn", "triton_fused_ln_rope_fn",
-    "set_attention_backward",
+    "set_attention_backward", "rope_cache_append_fn", "paged_decode_attn_func", "relative_position_bias_fn",
 ]
 
 _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
@@ -704,4 +706,247 @@ class FlashAttnFunc(torch.autograd.Function):
 
 def flash_attn_func(q, k, v, bias=None, causal=False, softmax_scale=None, return_lse=False, kernel_cache=None):
     o, lse = FlashAttnFunc.apply(q, k, v, bias, causal, softmax_scale, kernel_cache)
+    return (o, lse) if return_lse else o
+
+
+# ----------------------------------------------------------------------------------------------
+# learned relative position bias (no counterpart in the reference)
+# ----------------------------------------------------------------------------------------------
+
+
+class _RelativeRanges:
+    """The buckets as ranges of d = key position - query position, ascending (what the C ABI takes)."""
+
+    def __init__(self, starts, buckets):
+        self.starts, self.buckets, self.n = starts, buckets, len(starts)
+        self.c_starts = (ctypes.c_int32 * self.n)(*starts)
+        self.c_buckets = (ctypes.c_int32 * self.n)(*buckets)
+
+
+@functools.lru_cache(maxsize=64, typed=True)
+def relative_ranges(num_buckets, max_distance, bidirectional):
+    """Buckets of a learned relative position bias, n = query position - key position.  Causal (bidirectional False):
+    n < 0 counts as 0, and with e = num_buckets // 2 the distances n < e have a bucket each, the others
+    e + floor(log(n / e) / log(max_distance / e) * (num_buckets - e)), at most the last bucket.  Bidirectional: the same
+    with half of the buckets for n >= 0, and the other half, after them, for the keys behind the query with |n|.
+    The borders are found in whole numbers: bucket e + k begins at the smallest n with n^m >= max_distance^k e^(m - k), m the
+    number of logarithmic buckets, so no rounding of a logarithm decides a bucket."""
+    assert isinstance(num_buckets, int) and 2 <= num_buckets <= 256, f"{num_buckets=}: 2 to 256 buckets"
+    assert not bidirectional or (num_buckets % 2 == 0 and num_buckets >= 4), f"{num_buckets=}: bidirectional buckets are even, at least 4"
+    side = num_buckets // 2 if bidirectional else num_buckets
+    e = side // 2
+    assert isinstance(max_distance, int) and e < max_distance < 2**30, f"{max_distance=}: more than {e}, less than 2^30"
+    m = side - e
+    begin = list(range(e + 1))  # smallest n of buckets 0 .. e
+    for k in range(1, m):
+        bar = max_distance**k * e ** (m - k)
+        lo, hi = begin[-1], max_distance
+        while lo < hi:  # smallest n with n^m >= bar
+            mid = (lo + hi) // 2
+            lo, hi = (lo, mid) if mid**m >= bar else (mid + 1, hi)
+        begin.append(lo)
+    # a bucket that begins where the next one does holds nothing
+    held = [b for b in range(side) if b + 1 == side or begin[b] < begin[b + 1]]
+    starts, buckets = [], []
+    for b in reversed(held):  # keys in front of the query, farthest first: n from begin[b] on, d = -n up to -begin[b]
+        end = [begin[c] for c in held if c > b]
+        starts.append(1 - end[0] if end else -(2**31))
+        buckets.append(b)
+    if bidirectional:
+        for b in held:
+            if b > 0:
+                starts.append(begin[b])
+                buckets.append(side + b)
+    return _RelativeRanges(tuple(starts), tuple(buckets))
+
+
+def _same_device(what, device, *ts):
+    for t in ts:
+        if t is not None:
+            assert t.is_cuda, "rgd_triton_amd operators run on the GPU only"
+            assert t.device == device, f"{what}: tensors on {t.device} and {device}"
+
+
+def _on_device(device):
+    """Kernels are launched on the tensors' device, whichever is current."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+class Relative_Bias_Func(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, seqlen_q, seqlen_k, ranges, q_offset=0, dtype=None, kernel_cache=None):
+        dtype = dtype or weight.dtype
+        (weight,) = _lastdim_contig(weight)
+        if not _seen(kernel_cache, "fwd", _sig(weight) + (seqlen_q, seqlen_k, q_offset, dtype, ranges, weight.device)):
+            assert weight.is_cuda, "rgd_triton_amd operators run on the GPU only"
+            assert weight.dtype in _FLOATS and dtype in _FLOATS, "Only support fp16, bf16, and fp32"
+            assert weight.ndim == 2 and max(ranges.buckets) < weight.shape[0], f"{weight.shape=}"
+            assert seqlen_q >= 0 and seqlen_k >= 0, f"{seqlen_q=}, {seqlen_k=}"
+        num_buckets, nheads = weight.shape
+        bias = torch.empty((1, nheads, seqlen_q, seqlen_k), dtype=dtype, device=weight.device)
+        lib = _hip.lib()
+        with _on_device(weight.device):
+            _hip.check(lib.rgd_rel_bias_fwd(nheads, seqlen_q, seqlen_k, weight.data_ptr(), weight.stride(0), num_buckets,
+                                            _hip.dtype_code(weight.dtype), ranges.n, ranges.c_starts, ranges.c_buckets, q_offset,
+                                            t4(bias, True), _hip.dtype_code(dtype), _hip.stream_ptr(weight.device)),
+                       "rgd_rel_bias_fwd")
+        ctx.kernel_cache = kernel_cache
+        ctx.args = (num_buckets, nheads, seqlen_q, seqlen_k, ranges, q_offset, weight.dtype)
+        return bias
+
+    @staticmethod
+    def backward(ctx, dbias):
+        _no_capture("Relative_Bias_Func.backward")
+        num_buckets, nheads, seqlen_q, seqlen_k, ranges, q_offset, wdtype = ctx.args
+        (dbias,) = _lastdim_contig(dbias)
+        _seen(ctx.kernel_cache, "bwd", _sig(dbias))
+        dw = torch.empty((num_buckets, nheads), dtype=wdtype, device=dbias.device)
+        lib = _hip.lib()
+        nbytes = lib.rgd_rel_bias_bwd_workspace(nheads, seqlen_q, seqlen_k)
+        ws = _hip.workspace(dbias.device, nbytes)
+        with _on_device(dbias.device):
+            _hip.check(lib.rgd_rel_bias_bwd(nheads, seqlen_q, seqlen_k, t4(dbias, True), _hip.dtype_code(dbias.dtype), ranges.n,
+                                            ranges.c_starts, ranges.c_buckets, q_offset, dw.data_ptr(), nheads, num_buckets,
+                                            _hip.dtype_code(wdtype), ws.data_ptr(), nbytes, _hip.stream_ptr(dbias.device)),
+                       "rgd_rel_bias_bwd")
+        return dw, None, None, None, None, None, None
+
+
+def relative_position_bias_fn(weight, seqlen_q, seqlen_k, max_distance=128, bidirectional=True, q_offset=0, dtype=None,
+                              kernel_cache=None):
+    """Learned relative position bias for flash_attn_func(bias=...): (1, nheads, seqlen_q, seqlen_k) with
+    bias[0, h, i, j] = weight[bucket of key j for query i + q_offset, h], weight (num_buckets, nheads); the buckets are
+    relative_ranges'.  dtype: of the bias (the weight's by default; attention takes its own tensors' or fp32).  The
+    gradient of the weight is summed in fp32 and rounded once."""
+    return Relative_Bias_Func.apply(weight, seqlen_q, seqlen_k, relative_ranges(weight.shape[0], max_distance, bool(bidirectional)),
+                                    q_offset, dtype, kernel_cache)
+
+
+# ----------------------------------------------------------------------------------------------
+# paged key/value cache (no counterpart in the reference)
+# ----------------------------------------------------------------------------------------------
+
+
+def _no_grad(what, *ts):
+    assert not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)), \
+        f"{what} is for serving and has no gradient: call it under torch.no_grad()"
+
+
+def _check_cache(what, k_cache, v_cache, page_table, lens, batch, dtype, head_dim):
+    assert k_cache.ndim == 4 and k_cache.shape == v_cache.shape, f"{k_cache.shape=}, {v_cache.shape=}"
+    assert k_cache.stride(-1) == v_cache.stride(-1) == 1, f"{what}: the caches need unit-stride head dims"
+    assert k_cache.dtype == v_cache.dtype == dtype, f"All tensors must have the same type {dtype=}, {k_cache.dtype=}, {v_cache.dtype=}"
+    assert dtype in (torch.float16, torch.bfloat16), "Only support fp16 and bf16"
+    assert k_cache.shape[3] == head_dim <= 128, f"{what} only supports head dimensions up to 128, the cache's the same: {head_dim=}"
+    assert k_cache.shape[1] >= 1, f"{k_cache.shape=}: page size must be positive"
+    assert page_table.dtype == torch.int32 and page_table.ndim == 2 and page_table.shape[0] == batch, \
+        f"page_table is (batch, pages) int32: {page_table.dtype}, {page_table.shape}"
+    assert page_table.shape[1] <= 1 or page_table.stride(1) == 1, "page_table rows need unit stride"
+    _check_lens(lens, batch)
+
+
+def _check_lens(lens, batch):
+    assert lens.dtype == torch.int32 and lens.shape == (batch,) and (batch <= 1 or lens.stride(0) == 1), \
+        f"lengths are (batch,) int32, contiguous: {lens.dtype}, {lens.shape}"
+
+
+def _cache4(t):
+    # (num_pages, page_size, H, D) -> (page, head, slot) strides
+    return _hip.Tensor4(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1))
+
+
+def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens=None, seq_cutoff=None,
+                         heads_second=True, norm_eps=None, kernel_cache=None):
+    """Appends the new tokens of every sequence to a paged cache, rotating query and key at their positions on the way;
+    returns the rotated query, writes k_cache and v_cache in place.
+
+    query (B, Hq, T, D), key and value (B, Hkv, T, D) with heads_second, else (B, T, H, D); k_cache, v_cache
+    (num_pages, page_size, Hkv, D), any strides with a unit last one (head-major storage is passed as a transposed view);
+    page_table (B, pages) int32; cache_lens (B,) int32, the tokens already there: token t gets position cache_lens[b] + t, page
+    page_table[b, position // page_size].  new_lens (B,) int32: how many of the T tokens are real, the rest is padding (nothing
+    stored, query rows zero).  pos_emb as in triton_rope_fn, with a row for every position the page table covers; None: no
+    rotation.  Positions from seq_cutoff on (an int, or one for query and one for key) are not rotated.  norm_eps: LayerNorm over
+    the head dim in front of the rotation, as triton_fused_ln_rope_fn has it; None: none.  A token whose page number is outside
+    the cache is not stored; one whose position is outside the page table is padding.  cache_lens is the caller's to advance."""
+    what = "rope_cache_append"
+    query, key, value = _lastdim_contig(query, key, value)
+    if pos_emb is not None:
+        (pos_emb,) = _lastdim_contig(_table_for(pos_emb, query))
+    _no_grad(what, query, key, value, pos_emb, k_cache, v_cache)
+    head, tok = (1, 2) if heads_second else (2, 1)
+    sig = _sig(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens)
+    if not _seen(kernel_cache, "fwd", sig + (bool(heads_second), query.device)):
+        assert query.ndim == key.ndim == value.ndim == 4
+        assert query.dtype == key.dtype == value.dtype, "All tensors must have the same type"
+        batch, T, D = query.shape[0], query.shape[tok], query.shape[3]
+        assert key.shape == value.shape and (key.shape[0], key.shape[tok], key.shape[3]) == (batch, T, D), \
+            f"{query.shape=}, {key.shape=}, {value.shape=}"
+        _check_cache(what, k_cache, v_cache, page_table, cache_lens, batch, query.dtype, D)
+        assert k_cache.shape[2] == key.shape[head], f"{k_cache.shape=}, {key.shape=}"
+        if new_lens is not None:
+            _check_lens(new_lens, batch)
+        if pos_emb is not None:
+            assert pos_emb.ndim == 3 and pos_emb.shape[0] == 2 and pos_emb.dtype in _FLOATS, f"{pos_emb.shape=}"
+            assert pos_emb.shape[2] <= D and pos_emb.shape[2] % 2 == 0, f"{pos_emb.shape=}: an even rotary dim, at most {D=}"
+            assert pos_emb.shape[1] >= page_table.shape[1] * k_cache.shape[1], \
+                f"{pos_emb.shape=}: a row for every position of {page_table.shape[1]} pages of {k_cache.shape[1]}"
+        _same_device(what, query.device, query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens)
+    B, Hq, T, D = query.shape[0], query.shape[head], query.shape[tok], query.shape[3]
+    num_pages, page_size, Hkv, _ = k_cache.shape
+    if pos_emb is None:
+        pe = (None, 0, 0, 0, 0, _hip.RGD_F32)
+    else:
+        pe = (pos_emb.data_ptr(), pos_emb.shape[1], pos_emb.shape[2], pos_emb.stride(0), pos_emb.stride(1), _hip.dtype_code(pos_emb.dtype))
+    cq, ck = _cutoffs(seq_cutoff, 2**31 - 1, 2**31 - 1)
+    qo = torch.empty_like(query)
+    lib = _hip.lib()
+    with _on_device(query.device):
+        _hip.check(lib.rgd_rope_cache_append(
+            B, T, Hq, Hkv, D, t4(query, heads_second), t4(key, heads_second), t4(value, heads_second), t4(qo, heads_second),
+            _cache4(k_cache), _cache4(v_cache), num_pages, page_size, page_table.data_ptr(), page_table.shape[1],
+            page_table.stride(0), cache_lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(), *pe, cq, ck,
+            int(norm_eps is not None), float(norm_eps or 0.0), _hip.dtype_code(query.dtype), _hip.stream_ptr(query.device)),
+            "rgd_rope_cache_append")
+    torch.autograd.graph.increment_version((k_cache, v_cache))
+    return qo
+
+
+def paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight=None, max_distance=128, bidirectional=True,
+                           softmax_scale=None, return_lse=False, kernel_cache=None):
+    """Attention of one new token per sequence over a paged cache.
+
+    q (B, 1, Hq, D); k_cache, v_cache (num_pages, page_size, Hkv, D), Hq a multiple of Hkv (query head h reads key head
+    h // (Hq // Hkv)); page_table (B, pages) int32; seq_lens (B,) int32: keys 0 .. seq_lens[b] - 1 are seen, the new token's own
+    key among them.  rel_weight (num_buckets, Hq): the learned bias of relative_position_bias_fn for a query at position
+    seq_lens[b] - 1.  Returns o (B, 1, Hq, D), with return_lse also the logsumexp (B, Hq) in fp32.  A sequence without keys gives
+    o = 0, lse = -inf.  Keys on a page number outside the cache are not seen; lengths beyond the page table end there."""
+    what = "paged_decode_attn"
+    q, rel_weight = _lastdim_contig(q, rel_weight)
+    _no_grad(what, q, k_cache, v_cache, rel_weight)
+    if not _seen(kernel_cache, "fwd", _sig(q, k_cache, v_cache, page_table, seq_lens, rel_weight) + (q.device,)):
+        assert q.ndim == 4 and q.shape[1] == 1, f"{q.shape=}: one new token per sequence"
+        _check_cache(what, k_cache, v_cache, page_table, seq_lens, q.shape[0], q.dtype, q.shape[3])
+        assert k_cache.shape[2] >= 1 and q.shape[2] % k_cache.shape[2] == 0, f"{q.shape=}, {k_cache.shape=}: query heads in groups"
+        if rel_weight is not None:
+            assert rel_weight.ndim == 2 and rel_weight.shape[1] == q.shape[2] and rel_weight.dtype in _FLOATS, f"{rel_weight.shape=}"
+        _same_device(what, q.device, q, k_cache, v_cache, page_table, seq_lens, rel_weight)
+    B, _, Hq, D = q.shape
+    num_pages, page_size, Hkv, _ = k_cache.shape
+    softmax_scale = softmax_scale or 1.0 / math.sqrt(D)
+    rel = (None, 0, 0, _hip.RGD_F32, 0, None, None)
+    if rel_weight is not None:
+        r = relative_ranges(rel_weight.shape[0], max_distance, bool(bidirectional))
+        rel = (rel_weight.data_ptr(), rel_weight.stride(0), rel_weight.shape[0], _hip.dtype_code(rel_weight.dtype), r.n, r.c_starts,
+               r.c_buckets)
+    o = torch.empty((B, 1, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    lib = _hip.lib()
+    nbytes = lib.rgd_paged_decode_workspace(B, Hq, Hkv, D)
+    ws = _hip.workspace(q.device, nbytes)
+    with _on_device(q.device):
+        _hip.check(lib.rgd_paged_decode(
+            B, Hq, Hkv, D, t4(q, False), _cache4(k_cache), _cache4(v_cache), num_pages, page_size, page_table.data_ptr(),
+            page_table.shape[1], page_table.stride(0), seq_lens.data_ptr(), *rel, t4(o, False),
+            None if lse is None else lse.data_ptr(), _hip.dtype_code(q.dtype), float(softmax_scale), ws.data_ptr(), nbytes,
+            _hip.stream_ptr(q.device)), "rgd_paged_decode")
     return (o, lse) if return_lse else o

@@ -5,6 +5,9 @@ Reference: rgd_triton/ops.py:12-249.  Two defects of the reference are not repro
 FlashAttention module imports a module that does not exist (ops.py:37), and its RoPE module rotates
 query and key in place because the cache object lands in the in_place argument
 (rope/head_rope_cached.py:326-327); here FlashAttention works and RoPE is out of place.
+
+Beyond the reference: the learned relative position bias that FlashAttention takes (RelativePositionBias), and what the same
+model needs to run token by token (RoPECacheAppend / FusedLNRoPECacheAppend, PagedDecodeAttention).
 """
 import torch
 import torch.nn as nn
@@ -12,7 +15,8 @@ import torch.nn as nn
 from . import functional as F_
 
 __all__ = ["CachableModule", "FlashAttention", "L2Normalize", "FusedL2Normalize2", "FusedHeadLayerNorm",
-           "FusedRMSNorm", "FusedRMSNorm2", "RoPE", "FusedLNRoPE"]
+           "FusedRMSNorm", "FusedRMSNorm2", "RoPE", "FusedLNRoPE", "RelativePositionBias", "RoPECacheAppend",
+           "FusedLNRoPECacheAppend", "PagedDecodeAttention"]
 
 
 class CachableModule(nn.Module):
@@ -149,3 +153,57 @@ class FusedLNRoPE(CachableModule):
     def forward(self, query, key, pos_emb, seq_cutoff=None, heads_second=True, eps=1e-6):
         return self._triton_fn(query=query, key=key, pos_emb=pos_emb, seq_cutoff=seq_cutoff,
                                heads_second=heads_second, norm_eps=eps, kernel_cache=self.cache)
+
+
+class RelativePositionBias(CachableModule):
+    """Learned relative position bias: forward gives the (1, nheads, seqlen_q, seqlen_k) bias that FlashAttention takes."""
+
+    def __init__(self, num_buckets, nheads, max_distance=128, bidirectional=True, device=None, dtype=None):
+        super().__init__(cache_fields=("fwd", "bwd"))
+        self.max_distance = max_distance
+        self.bidirectional = bool(bidirectional)
+        F_.relative_ranges(num_buckets, max_distance, self.bidirectional)  # refuses impossible buckets
+        self.weight = nn.Parameter(torch.empty((num_buckets, nheads), device=device, dtype=dtype))
+        self.reset_parameters()
+        self._fn = F_.relative_position_bias_fn
+
+    def reset_parameters(self) -> None:
+        torch.nn.init.zeros_(self.weight)
+
+    def forward(self, seqlen_q, seqlen_k, q_offset=0, dtype=None):
+        return self._fn(self.weight, seqlen_q, seqlen_k, max_distance=self.max_distance, bidirectional=self.bidirectional,
+                        q_offset=q_offset, dtype=dtype, kernel_cache=self.cache)
+
+
+class RoPECacheAppend(CachableModule):
+    def __init__(self):
+        super().__init__(cache_fields=("fwd",))
+        self._fn = F_.rope_cache_append_fn
+
+    def forward(self, query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens=None, seq_cutoff=None,
+                heads_second=True):
+        return self._fn(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens=new_lens,
+                        seq_cutoff=seq_cutoff, heads_second=heads_second, kernel_cache=self.cache)
+
+
+class FusedLNRoPECacheAppend(CachableModule):
+    def __init__(self):
+        super().__init__(cache_fields=("fwd",))
+        self._fn = F_.rope_cache_append_fn
+
+    def forward(self, query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens=None, seq_cutoff=None,
+                heads_second=True, eps=1e-6):
+        return self._fn(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens=new_lens,
+                        seq_cutoff=seq_cutoff, heads_second=heads_second, norm_eps=eps, kernel_cache=self.cache)
+
+
+class PagedDecodeAttention(CachableModule):
+    def __init__(self):
+        super().__init__(cache_fields=("fwd",))
+        self._fn = F_.paged_decode_attn_func
+
+    def forward(self, q, k_cache, v_cache, page_table, seq_lens, rel_bias=None, softmax_scale=None):
+        """rel_bias: the RelativePositionBias the model was trained with, or None."""
+        rel = {} if rel_bias is None else dict(rel_weight=rel_bias.weight, max_distance=rel_bias.max_distance,
+                                               bidirectional=rel_bias.bidirectional)
+        return self._fn(q, k_cache, v_cache, page_table, seq_lens, softmax_scale=softmax_scale, kernel_cache=self.cache, **rel)
