@@ -315,8 +315,8 @@ int rgd_attn_bwd(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t D,
  * A cache is (num_pages, H, page_size, D) given as (page, head, slot) strides in an rgd_tensor4 (stride_b = page),
  * so that token-major and head-major storage are both views of it; keys and values have separate descriptors of the
  * same sizes.  Position t of sequence b lives in page page_table[b * table_stride + t / page_size], slot t % page_size;
- * page_table and the length arrays are int32 device memory.  Positions lie in [0, max_pages * page_size), which must
- * be below 2^31.  A page number outside [0, num_pages) is no page: such a token is not stored, such a key not seen.
+ * page_table and the length arrays are int32 device memory.  Positions lie in [0, max_pages * page_size), at most
+ * 2^31 - 1024 of them.  A page number outside [0, num_pages) is no page: such a token is not stored, such a key not seen.
  * fp16 or bf16, D <= 128; any strides, 16-byte accesses where pointers, strides, D and R allow them.
  * ------------------------------------------------------------------------------------------ */
 

@@ -156,7 +156,7 @@ extern "C" int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t H
     RGD_REQUIRE(D >= 1 && D <= 128, RGD_ERR_INVALID, "%s: Only supports head dimensions up to 128", name);
     RGD_REQUIRE(page_size >= 1, RGD_ERR_INVALID, "%s: page size must be positive", name);
     const int64_t lim = int64_t(1) << 31;
-    RGD_REQUIRE(num_pages < lim && page_size < lim && max_pages < lim && max_pages * page_size < lim, RGD_ERR_UNSUPPORTED,
+    RGD_REQUIRE(num_pages < lim && page_size < lim && max_pages < lim && max_pages * page_size <= lim - 1024, RGD_ERR_UNSUPPORTED,
                 "%s: more than 2^31 positions or pages", name);
     RGD_REQUIRE(B < lim && T < lim && Hq < lim && Hkv < lim, RGD_ERR_UNSUPPORTED, "%s: more than 2^31 rows", name);
     if (B == 0 || T == 0 || Hq + Hkv == 0) return RGD_OK;

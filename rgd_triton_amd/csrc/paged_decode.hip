@@ -1,97 +1,34 @@
-// Attention of one new token per sequence over a paged key/value cache.
-//
-//   s_j = softmax_scale q . k_j (+ W[bucket(j - (len - 1))][h]),  o = sum_j softmax(s)_j v_j,  lse = log sum_j exp(s_j)
-//
-// Simple form: a workgroup per (sequence, query head), a wavefront per key in turn, one pass with a running maximum and sum.
-#include "common.h"
+// Host side of the single-token attention over a paged cache: validation, choice of the kernel variant, entry points.
+#include "paged_decode.h"
 
 #include <string.h>
 
 namespace {
 
-constexpr int MAX_RANGES = 256;
+// Workgroups of the decode launch: DEC_WAVES_PER_SIMD resident on every compute unit.
+constexpr int DEC_WAVES_PER_SIMD = 2;
+int64_t decode_grid() { return (int64_t)rgd_num_cus() * DEC_WAVES_PER_SIMD; }
 
-struct DecodeParams {
-    const void* q;
-    const void* k;
-    const void* v;
-    void* o;
-    float* lse;
-    int64_t sq[2], so[2], sk[3], sv[3];  // (batch, head); (page, head, slot)
-    const int32_t* page_table;
-    const int32_t* seq_lens;
-    int64_t table_stride;
-    int64_t capacity;
-    int B, Hq, group, D, num_pages;
-    FastDiv div_page;
-    float scale;
-    const void* w;  // (buckets, Hq) or null
-    int64_t w_stride;
-    int w_dtype, n_ranges;
-    int start[MAX_RANGES], bucket[MAX_RANGES];
-};
+int chunks_of(int64_t D) { return (int)((D + 31) / 32); }
 
-__device__ __forceinline__ float load_dyn(const void* p, int dtype, int64_t i) {
-    if (dtype == RGD_BF16) return to_f32(static_cast<const bf16_t*>(p)[i]);
-    if (dtype == RGD_F16) return to_f32(static_cast<const f16_t*>(p)[i]);
-    return static_cast<const float*>(p)[i];
+template <typename T, int NC, bool PAGE8, bool SMALL>
+int decode_launch(const DecodeParams& p, unsigned grid, bool merge, hipStream_t s) {
+    const hipError_t e = p.w ? rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, true>, dim3(grid), dim3(256), 0, s, p)
+                             : rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, false>, dim3(grid), dim3(256), 0, s, p);
+    const int rc = rgd_launch_status("rgd_paged_decode", e);
+    if (rc != RGD_OK || !merge) return rc;
+    return rgd_launch_status("rgd_paged_decode", rgd_launch(paged_decode_merge_kernel<T, NC, SMALL>, dim3((unsigned)p.B * (unsigned)p.Hq),
+                                                            dim3(256), 0, s, p));
 }
 
-template <typename T> __global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p) {
-    __shared__ float sm[4], sl[4], so[4][128];
-    const int lane = lane_id(), wave = threadIdx.x >> 6;
-    const int b = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
-    const int hk = h / p.group;
-    const int D = p.D;
-    const int64_t want = p.seq_lens[b];
-    const int len = (int)(want < 0 ? 0 : (want < p.capacity ? want : p.capacity));
-    const T* q = static_cast<const T*>(p.q) + b * p.sq[0] + h * p.sq[1];
-    const int d0 = lane * 2, d1 = lane * 2 + 1;
-    const float q0 = d0 < D ? to_f32(q[d0]) : 0.f, q1 = d1 < D ? to_f32(q[d1]) : 0.f;
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int j = wave; j < len; j += 4) {
-        const uint32_t entry = fast_div(j, p.div_page);
-        const int page = p.page_table[b * p.table_stride + entry];
-        if (page < 0 || page >= p.num_pages) continue;  // no such page: the key is absent
-        const uint32_t slot = j - entry * p.div_page.d;
-        const T* k = static_cast<const T*>(p.k) + page * p.sk[0] + hk * p.sk[1] + slot * p.sk[2];
-        const T* v = static_cast<const T*>(p.v) + page * p.sv[0] + hk * p.sv[1] + slot * p.sv[2];
-        float s = (d0 < D ? q0 * to_f32(k[d0]) : 0.f) + (d1 < D ? q1 * to_f32(k[d1]) : 0.f);
-        s = group_reduce<64>(s) * p.scale;
-        if (p.w) {
-            const int d = j - (len - 1);
-            int r = 0;
-            while (r + 1 < p.n_ranges && d >= p.start[r + 1]) ++r;
-            s += load_dyn(p.w, p.w_dtype, p.bucket[r] * p.w_stride + h);
-        }
-        const float nm = fmaxf(m, s);
-        const float ref = nm == -INFINITY ? 0.f : nm;
-        const float alpha = expf(m - ref), e = expf(s - ref);
-        l = l * alpha + e;
-        o0 = o0 * alpha + e * (d0 < D ? to_f32(v[d0]) : 0.f);
-        o1 = o1 * alpha + e * (d1 < D ? to_f32(v[d1]) : 0.f);
-        m = nm;
-    }
-    sm[wave] = m;
-    sl[wave] = l;
-    so[wave][d0] = o0;
-    so[wave][d1] = o1;
-    __syncthreads();
-    if (wave == 0) {
-        float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-        const float ref = top == -INFINITY ? 0.f : top;
-        float total = 0.f, a0 = 0.f, a1 = 0.f;
-        for (int w = 0; w < 4; ++w) {
-            const float f = expf(sm[w] - ref);
-            total += f * sl[w];
-            a0 += f * so[w][d0];
-            a1 += f * so[w][d1];
-        }
-        const float inv = total == 0.f ? 0.f : 1.0f / total;
-        T* o = static_cast<T*>(p.o) + b * p.so[0] + h * p.so[1];
-        if (d0 < D) o[d0] = from_f32<T>(a0 * inv);
-        if (d1 < D) o[d1] = from_f32<T>(a1 * inv);
-        if (p.lse && lane == 0) p.lse[(int64_t)b * p.Hq + h] = total == 0.f ? -INFINITY : ref + logf(total);
+template <typename T> int decode_dispatch(const DecodeParams& p, unsigned grid, bool merge, hipStream_t s) {
+    if (p.D < 8) return decode_launch<T, 1, false, true>(p, grid, merge, s);
+    const bool page8 = p.div_page.d % 8 == 0;
+    switch (chunks_of(p.D)) {
+        case 1: return page8 ? decode_launch<T, 1, true, false>(p, grid, merge, s) : decode_launch<T, 1, false, false>(p, grid, merge, s);
+        case 2: return page8 ? decode_launch<T, 2, true, false>(p, grid, merge, s) : decode_launch<T, 2, false, false>(p, grid, merge, s);
+        case 3: return page8 ? decode_launch<T, 3, true, false>(p, grid, merge, s) : decode_launch<T, 3, false, false>(p, grid, merge, s);
+        default: return page8 ? decode_launch<T, 4, true, false>(p, grid, merge, s) : decode_launch<T, 4, false, false>(p, grid, merge, s);
     }
 }
 
@@ -100,8 +37,10 @@ template <typename T> __global__ __launch_bounds__(256) void paged_decode_kernel
 extern "C" {
 
 size_t rgd_paged_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
-    (void)B, (void)Hq, (void)Hkv, (void)D;
-    return 0;
+    if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || D > 128) return 0;
+    const int64_t group = Hq / Hkv, units = Hkv * ((group + 15) / 16), rows = group < 16 ? group : 16;
+    const int64_t plan = (B * units * (int64_t)sizeof(int2) + 15) / 16 * 16;
+    return (size_t)(plan + 2 * decode_grid() * (rows * 32 * chunks_of(D) + 32) * 4);
 }
 
 int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_tensor4* q, const rgd_tensor4* k_cache,
@@ -117,7 +56,7 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
     RGD_REQUIRE(D >= 1 && D <= 128, RGD_ERR_INVALID, "%s: Only supports head dimensions up to 128", name);
     RGD_REQUIRE(page_size >= 1, RGD_ERR_INVALID, "%s: page size must be positive", name);
     const int64_t lim = int64_t(1) << 31;
-    RGD_REQUIRE(num_pages < lim && page_size < lim && max_pages < lim && max_pages * page_size < lim, RGD_ERR_UNSUPPORTED,
+    RGD_REQUIRE(num_pages < lim && page_size < lim && max_pages < lim && max_pages * page_size <= lim - 1024, RGD_ERR_UNSUPPORTED,
                 "%s: more than 2^31 positions or pages", name);
     RGD_REQUIRE(B < lim && Hq < lim && B * Hq < lim, RGD_ERR_UNSUPPORTED, "%s: more than 2^31 rows", name);
     if (B == 0 || Hq == 0) return RGD_OK;
@@ -130,7 +69,7 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
     memset(&p, 0, sizeof(p));
     if (rel_weight) {
         RGD_REQUIRE(rgd_dtype_ok(w_dtype), RGD_ERR_INVALID, "%s: Only support fp16, bf16, and fp32 bias weights", name);
-        RGD_REQUIRE(n_ranges >= 1 && n_ranges <= MAX_RANGES && starts && buckets, RGD_ERR_INVALID, "%s: 1 to %d ranges", name, MAX_RANGES);
+        RGD_REQUIRE(n_ranges >= 1 && n_ranges <= DEC_MAX_RANGES && starts && buckets, RGD_ERR_INVALID, "%s: 1 to %d ranges", name, DEC_MAX_RANGES);
         for (int64_t i = 0; i < n_ranges; ++i) {
             RGD_REQUIRE(buckets[i] >= 0 && buckets[i] < num_buckets, RGD_ERR_INVALID, "%s: a bucket outside the weight", name);
             p.start[i] = starts[i];
@@ -155,20 +94,28 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
     p.page_table = page_table;
     p.seq_lens = seq_lens;
     p.table_stride = table_stride;
-    p.capacity = none ? 0 : max_pages * page_size;
+    p.capacity = none ? 0 : (int)(max_pages * page_size);
     p.B = (int)B;
+    p.Hkv = (int)Hkv;
     p.Hq = (int)Hq;
     p.group = (int)(Hq / Hkv);
+    p.head_tiles = (p.group + 15) / 16;
+    p.units = p.Hkv * p.head_tiles;
+    p.part_rows = p.group < 16 ? p.group : 16;
     p.D = (int)D;
     p.num_pages = (int)num_pages;
     p.div_page = make_fastdiv((uint32_t)page_size);
     p.scale = softmax_scale;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    (void)workspace, (void)workspace_bytes;
-    const dim3 grid((unsigned)(B * Hq));
-    const hipError_t e = dtype == RGD_F16 ? rgd_launch(paged_decode_kernel<f16_t>, grid, dim3(256), 0, s, p)
-                                          : rgd_launch(paged_decode_kernel<bf16_t>, grid, dim3(256), 0, s, p);
-    return rgd_launch_status(name, e);
+    RGD_REQUIRE(workspace && workspace_bytes >= rgd_paged_decode_workspace(B, Hq, Hkv, D), RGD_ERR_WORKSPACE,
+                "%s: workspace of %zu bytes, needs %zu", name, workspace_bytes, rgd_paged_decode_workspace(B, Hq, Hkv, D));
+    p.plan = static_cast<int2*>(workspace);
+    p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (B * p.units * (int64_t)sizeof(int2) + 15) / 16 * 16);
+    // more workgroups than there can be tiles have nothing to do; units of one tile are in no two workgroups
+    const int64_t most = p.capacity > DEC_TILE ? (p.capacity + DEC_TILE - 1) / DEC_TILE : 1;
+    const int64_t tiles = B * p.units * most;
+    const unsigned grid = (unsigned)(tiles < decode_grid() ? tiles : decode_grid());
+    return dtype == RGD_F16 ? decode_dispatch<f16_t>(p, grid, most > 1, s) : decode_dispatch<bf16_t>(p, grid, most > 1, s);
 }
 
 }  // extern "C"

@@ -41,13 +41,14 @@ def check_decode(o, lse, ref, length, D, name=""):
     """o and lse against the oracle's.  In 32 bits a logit's product is off by at most d = (D + 4) 2^-24 reach (D products of
     16-bit values, exact, and their sums; the scale), the logit itself by 2 roundings of its value (bias, difference to the
     maximum), the exponential by 4 2^-24 relative: every p by r = d + 2^-22 |logit| + 2^-22 relative, numerator and denominator
-    both; p split in two 16-bit parts is off by 2^-16 at most; sums over the keys add length 2^-24.  The output is then
+    both; p is split into two 16-bit parts, the first within 2^-8 of (1 - 2^-7) p (bf16), so that the second is at most
+    (2^-7 + 2^-8) p = 0.0118 p and its own rounding at most 2^-8 0.0118 p < 2^-14 p; sums over the keys add length 2^-24.  The output is then
     rounded once."""
     ro, rlse, weighted, reach = ref
     span = reach.max().item() + rlse[torch.isfinite(rlse)].abs().max().item() if torch.isfinite(rlse).any() else 0.0
     r = (D + 4) * 2.0**-24 * reach + 2.0**-22 * (span + 1)
     sums = (length + 16) * 2.0**-24
-    rounded_once(o, ro, (2 * r + 2 * sums + 2.0**-16)[:, None, :, None] * weighted, f"{name} o")
+    rounded_once(o, ro, (2 * r + 2 * sums + 2.0**-14)[:, None, :, None] * weighted, f"{name} o")
     if lse is not None:
         a = lse.cpu().double()
         fin = torch.isfinite(rlse)

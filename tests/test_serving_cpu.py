@@ -133,6 +133,8 @@ def test_decode_refusals():
     assert _decode(**{**rel, "wdt": 7}) == -1 and b"bias weights" in err()
     assert _decode(**{**rel, "nb": 2}) == -1 and b"bucket outside" in err()
     assert _decode(**{**rel, "n": 0}) == -1 and _decode(**{**rel, "n": 257}) == -1 and _decode(**{**rel, "starts": None}) == -1
+    need = _hip.lib().rgd_paged_decode_workspace(1, 4, 2, 64)
+    assert need > 0 and _decode(bytes=need - 1) == -4 and b"workspace" in err() and _decode(work=None) == -4
     assert _decode(B=0) == 0 and _decode(Hq=0, Hkv=1) == 0
 
 
