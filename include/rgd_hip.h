@@ -368,7 +368,7 @@ int rgd_rel_bias_fwd(int64_t H, int64_t Tq, int64_t Tk, const void* weight, int6
 
 /* dweight[b * dw_stride + h] = sum of dbias[h, i, j] over the pairs whose d lies in bucket b (0 for a bucket without a range):
  * fp32 sums in a fixed order, rounded once to the weight's type.  Scratch: any contents on entry, 16-byte aligned. */
-size_t rgd_rel_bias_bwd_workspace(int64_t H, int64_t Tq, int64_t Tk);
+size_t rgd_rel_bias_bwd_workspace(int64_t H, int64_t Tq, int64_t Tk, int64_t num_buckets);
 int rgd_rel_bias_bwd(int64_t H, int64_t Tq, int64_t Tk, const rgd_tensor4* dbias, int dbias_dtype,
                      int64_t n_ranges, const int32_t* starts, const int32_t* buckets, int64_t q_offset,
                      void* dweight, int64_t dw_stride, int64_t num_buckets, int dw_dtype,

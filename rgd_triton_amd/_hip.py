@@ -74,7 +74,7 @@ _SIGNATURES = {
     "rgd_paged_decode": (_int, [_i64] * 4 + [_T4] * 3 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, _i64, _vp, _vp,
                                                          _T4, _vp, _int, _f32, _vp, _sz, _vp]),
     "rgd_rel_bias_fwd": (_int, [_i64] * 3 + [_vp, _i64, _i64, _int, _i64, _vp, _vp, _i64, _T4, _int, _vp]),
-    "rgd_rel_bias_bwd_workspace": (_sz, [_i64] * 3),
+    "rgd_rel_bias_bwd_workspace": (_sz, [_i64] * 4),
     "rgd_rel_bias_bwd": (_int, [_i64] * 3 + [_T4, _int, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _int, _vp, _sz, _vp]),
 }
 

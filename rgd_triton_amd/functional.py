@@ -802,7 +802,7 @@ class Relative_Bias_Func(torch.autograd.Function):
         _seen(ctx.kernel_cache, "bwd", _sig(dbias))
         dw = torch.empty((num_buckets, nheads), dtype=wdtype, device=dbias.device)
         lib = _hip.lib()
-        nbytes = lib.rgd_rel_bias_bwd_workspace(nheads, seqlen_q, seqlen_k)
+        nbytes = lib.rgd_rel_bias_bwd_workspace(nheads, seqlen_q, seqlen_k, num_buckets)
         ws = _hip.workspace(dbias.device, nbytes)
         with _on_device(dbias.device):
             _hip.check(lib.rgd_rel_bias_bwd(nheads, seqlen_q, seqlen_k, t4(dbias, True), _hip.dtype_code(dbias.dtype), ranges.n,

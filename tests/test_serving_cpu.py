@@ -164,7 +164,7 @@ def test_rel_bias_refusals():
         assert f(H=0) == 0
     assert fwd(w=None) == -1 and fwd(bias=None) == -1 and bwd(d=None) == -1 and bwd(dw=None) == -1
     assert bwd(bytes=16) == -4 and b"workspace" in err()
-    assert lib.rgd_rel_bias_bwd_workspace(0, 5, 5) == 0 and lib.rgd_rel_bias_bwd_workspace(3, 5, 5) > 0
+    assert lib.rgd_rel_bias_bwd_workspace(0, 5, 5, 8) == 0 and lib.rgd_rel_bias_bwd_workspace(3, 5, 5, 8) > 0
     assert fwd(Tq=0) == 0
 
 
