@@ -6,6 +6,7 @@ There is no fallback path: if the library is missing, every operator raises.
 import ctypes
 import os
 import re
+import struct
 import threading
 import warnings
 
@@ -36,7 +37,8 @@ class Tensor4(ctypes.Structure):
 _i64, _int, _f32, _vp, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 _T3, _T4 = ctypes.POINTER(Tensor3), ctypes.POINTER(Tensor4)
 
-# argument types of every entry point, in the order of include/rgd_hip.h
+# argument types of every entry point, in the order of include/rgd_hip.h (the operators that a serving loop calls token by
+# token take their tensor descriptors as packed bytes, see desc4: half of the host time of building and converting structures)
 _SIGNATURES = {
     "rgd_version": (_int, []),
     "rgd_last_error": (ctypes.c_char_p, []),
@@ -68,14 +70,14 @@ _SIGNATURES = {
     "rgd_attn_bwd_workspace": (_sz, [_i64] * 5 + [_int]),
     "rgd_attn_bwd": (_int, [_i64] * 5 + [_T4] * 5 + [_vp] + [_T4, _int, _int] + [_T4] * 4 + [_int, _int, _f32, _int, _vp,
                                                                                          _vp, _sz, _vp]),
-    "rgd_rope_cache_append": (_int, [_i64] * 5 + [_T4] * 6 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp] + [_i64] * 4 +
+    "rgd_rope_cache_append": (_int, [_i64] * 5 + [_vp] * 6 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp] + [_i64] * 4 +
                               [_int, _i64, _i64, _int, _f32, _int, _vp]),
     "rgd_paged_decode_workspace": (_sz, [_i64] * 4),
-    "rgd_paged_decode": (_int, [_i64] * 4 + [_T4] * 3 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, _i64, _vp, _vp,
-                                                         _T4, _vp, _int, _f32, _vp, _sz, _vp]),
-    "rgd_rel_bias_fwd": (_int, [_i64] * 3 + [_vp, _i64, _i64, _int, _i64, _vp, _vp, _i64, _T4, _int, _vp]),
+    "rgd_paged_decode": (_int, [_i64] * 4 + [_vp] * 3 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, _i64, _vp, _vp,
+                                                         _vp, _vp, _int, _f32, _vp, _sz, _vp]),
+    "rgd_rel_bias_fwd": (_int, [_i64] * 3 + [_vp, _i64, _i64, _int, _i64, _vp, _vp, _i64, _vp, _int, _vp]),
     "rgd_rel_bias_bwd_workspace": (_sz, [_i64] * 4),
-    "rgd_rel_bias_bwd": (_int, [_i64] * 3 + [_T4, _int, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _int, _vp, _sz, _vp]),
+    "rgd_rel_bias_bwd": (_int, [_i64] * 3 + [_vp, _int, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _int, _vp, _sz, _vp]),
 }
 
 _lib = None
@@ -142,6 +144,10 @@ def t4(t, heads_second):
     if heads_second:
         return Tensor4(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
     return Tensor4(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1))
+
+
+# an rgd_tensor4 as bytes, accepted where an entry point's argument is declared void*: (pointer, stride_b, stride_h, stride_n)
+desc4 = struct.Struct("@Pqqq").pack
 
 
 def stream_ptr(device):

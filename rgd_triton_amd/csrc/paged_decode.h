@@ -26,6 +26,8 @@
 
 #include "attn_common.h"
 
+#include <type_traits>
+
 constexpr int DEC_MAX_RANGES = 256;
 constexpr int DEC_TILE = 128;  // keys of a scheduling tile: 4 wavefronts x 32
 
@@ -47,11 +49,15 @@ struct DecodeParams {
     int2* plan;        // per unit of the batch: workgroups its first and last piece are in
     float* part;       // two slots per workgroup: O [rows][DP], then m [16], l [16]
     int part_rows;     // query heads of a slot
-    const void* w;     // relative bias (buckets, Hq)
+};
+
+struct DecodeBias {  // relative bias: weight (buckets, Hq), ranges of the distance and their buckets
+    const void* w;
     int64_t w_stride;
     int w_dtype, n_ranges;
     int start[DEC_MAX_RANGES], bucket[DEC_MAX_RANGES];
 };
+struct DecodeNoBias {};  // (2 KB less to hand over with every launch)
 
 template <typename T> struct Mfma16;
 template <> struct Mfma16<bf16_t> {
@@ -94,7 +100,8 @@ struct DecodePiece {
 // NC: 32-channel chunks of the head dim (DP = 32 NC).  PAGE8: the page size is a multiple of 8, so the 8 keys of a lane group
 // stand in one page (one lookup instead of 8).  SMALL: D < 8, rows are read element by element.
 template <typename T, int NC, bool PAGE8, bool SMALL, bool BIAS>
-__global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p) {
+__global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p,
+                                                           const std::conditional_t<BIAS, DecodeBias, DecodeNoBias> rel) {
     constexpr int DP = 32 * NC, VE = DP / 16, VW = VE / 2, OSTRIDE = DP + 4;
     __shared__ float s_o[4][16][OSTRIDE];
     __shared__ float s_m[4][16], s_l[4][16];
@@ -166,8 +173,8 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p)
     while (x < x_end) {
         const int len = __builtin_amdgcn_readfirstlane(length(b));
         const int ntiles = tiles_of(len);
-        const int64_t rel = x - base;
-        const int unit = (int)(rel / ntiles), tile0 = (int)(rel - (int64_t)unit * ntiles);
+        const int64_t in_seq = x - base;
+        const int unit = (int)(in_seq / ntiles), tile0 = (int)(in_seq - (int64_t)unit * ntiles);
         const int tile1 = (int)min((int64_t)ntiles, tile0 + (x_end - x));
         const int t_end = min(len, tile1 * DEC_TILE);
         const int hk = unit / p.head_tiles, head0 = hk * p.group + (unit - hk * p.head_tiles) * 16;
@@ -175,16 +182,16 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p)
 
         if constexpr (BIAS) {
             __syncthreads();
-            for (int i = tid; i < p.n_ranges * 16; i += 256) {
+            for (int i = tid; i < rel.n_ranges * 16; i += 256) {
                 const int r = i >> 4, h = i & 15;
                 float wv = 0.f;
                 if (h < heads) {
-                    const int64_t at = p.bucket[r] * p.w_stride + head0 + h;
-                    wv = p.w_dtype == RGD_F32 ? static_cast<const float*>(p.w)[at]
-                         : p.w_dtype == RGD_F16 ? to_f32(static_cast<const f16_t*>(p.w)[at]) : to_f32(static_cast<const bf16_t*>(p.w)[at]);
+                    const int64_t at = rel.bucket[r] * rel.w_stride + head0 + h;
+                    wv = rel.w_dtype == RGD_F32 ? static_cast<const float*>(rel.w)[at]
+                         : rel.w_dtype == RGD_F16 ? to_f32(static_cast<const f16_t*>(rel.w)[at]) : to_f32(static_cast<const bf16_t*>(rel.w)[at]);
                 }
                 s_w[r][h] = wv;
-                if (h == 0) s_start[r] = r == 0 ? INT32_MIN : p.start[r];
+                if (h == 0) s_start[r] = r == 0 ? INT32_MIN : rel.start[r];
             }
             __syncthreads();
         }
@@ -305,12 +312,12 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p)
             for (int i = 0; i < 8; ++i) x8[i] = s[i >> 2][i & 3] * p.scale;
             if constexpr (BIAS) {
                 const int d0 = t + 8 * g - (len - 1);
-                if (t + 31 - (len - 1) < s_start[min(1, p.n_ranges - 1)]) {  // all in the first range
+                if (t + 31 - (len - 1) < s_start[min(1, rel.n_ranges - 1)]) {  // all in the first range
                     const float wv = s_w[0][n16];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x8[i] += wv;
                 } else {
-                    int lo = 0, hi = p.n_ranges - 1;  // last range that begins at or before d0
+                    int lo = 0, hi = rel.n_ranges - 1;  // last range that begins at or before d0
                     while (lo < hi) {
                         const int mid = (lo + hi + 1) >> 1;
                         if (s_start[mid] <= d0) lo = mid;
@@ -318,7 +325,7 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p)
                     }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        while (lo + 1 < p.n_ranges && s_start[lo + 1] <= d0 + i) ++lo;
+                        while (lo + 1 < rel.n_ranges && s_start[lo + 1] <= d0 + i) ++lo;
                         x8[i] += s_w[lo][n16];
                     }
                 }

@@ -12,23 +12,23 @@ int64_t decode_grid() { return (int64_t)rgd_num_cus() * DEC_WAVES_PER_SIMD; }
 int chunks_of(int64_t D) { return (int)((D + 31) / 32); }
 
 template <typename T, int NC, bool PAGE8, bool SMALL>
-int decode_launch(const DecodeParams& p, unsigned grid, bool merge, hipStream_t s) {
-    const hipError_t e = p.w ? rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, true>, dim3(grid), dim3(256), 0, s, p)
-                             : rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, false>, dim3(grid), dim3(256), 0, s, p);
+int decode_launch(const DecodeParams& p, const DecodeBias* rel, unsigned grid, bool merge, hipStream_t s) {
+    const hipError_t e = rel ? rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, true>, dim3(grid), dim3(256), 0, s, p, *rel)
+                             : rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, false>, dim3(grid), dim3(256), 0, s, p, DecodeNoBias{});
     const int rc = rgd_launch_status("rgd_paged_decode", e);
     if (rc != RGD_OK || !merge) return rc;
     return rgd_launch_status("rgd_paged_decode", rgd_launch(paged_decode_merge_kernel<T, NC, SMALL>, dim3((unsigned)p.B * (unsigned)p.Hq),
                                                             dim3(256), 0, s, p));
 }
 
-template <typename T> int decode_dispatch(const DecodeParams& p, unsigned grid, bool merge, hipStream_t s) {
-    if (p.D < 8) return decode_launch<T, 1, false, true>(p, grid, merge, s);
+template <typename T> int decode_dispatch(const DecodeParams& p, const DecodeBias* rel, unsigned grid, bool merge, hipStream_t s) {
+    if (p.D < 8) return decode_launch<T, 1, false, true>(p, rel, grid, merge, s);
     const bool page8 = p.div_page.d % 8 == 0;
     switch (chunks_of(p.D)) {
-        case 1: return page8 ? decode_launch<T, 1, true, false>(p, grid, merge, s) : decode_launch<T, 1, false, false>(p, grid, merge, s);
-        case 2: return page8 ? decode_launch<T, 2, true, false>(p, grid, merge, s) : decode_launch<T, 2, false, false>(p, grid, merge, s);
-        case 3: return page8 ? decode_launch<T, 3, true, false>(p, grid, merge, s) : decode_launch<T, 3, false, false>(p, grid, merge, s);
-        default: return page8 ? decode_launch<T, 4, true, false>(p, grid, merge, s) : decode_launch<T, 4, false, false>(p, grid, merge, s);
+        case 1: return page8 ? decode_launch<T, 1, true, false>(p, rel, grid, merge, s) : decode_launch<T, 1, false, false>(p, rel, grid, merge, s);
+        case 2: return page8 ? decode_launch<T, 2, true, false>(p, rel, grid, merge, s) : decode_launch<T, 2, false, false>(p, rel, grid, merge, s);
+        case 3: return page8 ? decode_launch<T, 3, true, false>(p, rel, grid, merge, s) : decode_launch<T, 3, false, false>(p, rel, grid, merge, s);
+        default: return page8 ? decode_launch<T, 4, true, false>(p, rel, grid, merge, s) : decode_launch<T, 4, false, false>(p, rel, grid, merge, s);
     }
 }
 
@@ -67,18 +67,21 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
     RGD_REQUIRE(q && q->ptr && o && o->ptr, RGD_ERR_INVALID, "%s: null tensor", name);
     DecodeParams p;
     memset(&p, 0, sizeof(p));
+    DecodeBias rel;
+    const DecodeBias* bias = nullptr;
     if (rel_weight) {
         RGD_REQUIRE(rgd_dtype_ok(w_dtype), RGD_ERR_INVALID, "%s: Only support fp16, bf16, and fp32 bias weights", name);
         RGD_REQUIRE(n_ranges >= 1 && n_ranges <= DEC_MAX_RANGES && starts && buckets, RGD_ERR_INVALID, "%s: 1 to %d ranges", name, DEC_MAX_RANGES);
         for (int64_t i = 0; i < n_ranges; ++i) {
             RGD_REQUIRE(buckets[i] >= 0 && buckets[i] < num_buckets, RGD_ERR_INVALID, "%s: a bucket outside the weight", name);
-            p.start[i] = starts[i];
-            p.bucket[i] = buckets[i];
+            rel.start[i] = starts[i];
+            rel.bucket[i] = buckets[i];
         }
-        p.w = rel_weight;
-        p.w_stride = w_stride;
-        p.w_dtype = w_dtype;
-        p.n_ranges = (int)n_ranges;
+        rel.w = rel_weight;
+        rel.w_stride = w_stride;
+        rel.w_dtype = w_dtype;
+        rel.n_ranges = (int)n_ranges;
+        bias = &rel;
     }
     p.q = q->ptr;
     p.o = o->ptr;
@@ -115,7 +118,7 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
     const int64_t most = p.capacity > DEC_TILE ? (p.capacity + DEC_TILE - 1) / DEC_TILE : 1;
     const int64_t tiles = B * p.units * most;
     const unsigned grid = (unsigned)(tiles < decode_grid() ? tiles : decode_grid());
-    return dtype == RGD_F16 ? decode_dispatch<f16_t>(p, grid, most > 1, s) : decode_dispatch<bf16_t>(p, grid, most > 1, s);
+    return dtype == RGD_F16 ? decode_dispatch<f16_t>(p, bias, grid, most > 1, s) : decode_dispatch<bf16_t>(p, bias, grid, most > 1, s);
 }
 
 }  // extern "C"

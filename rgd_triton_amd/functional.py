@@ -18,7 +18,6 @@ Differences from the reference, all deliberate:
     signatures instead of a compiled-kernel handle, so a change of shape, dtype or bias kind after
     the first call can never reuse a stale specialisation.
 """
-import contextlib
 import ctypes
 import functools
 import math
@@ -718,7 +717,7 @@ class _RelativeRanges:
     """The buckets as ranges of d = key position - query position, ascending (what the C ABI takes)."""
 
     def __init__(self, starts, buckets):
-        self.starts, self.buckets, self.n = starts, buckets, len(starts)
+        self.starts, self.buckets, self.n, self.most = starts, buckets, len(starts), max(buckets)
         self.c_starts = (ctypes.c_int32 * self.n)(*starts)
         self.c_buckets = (ctypes.c_int32 * self.n)(*buckets)
 
@@ -760,56 +759,71 @@ def relative_ranges(num_buckets, max_distance, bidirectional):
     return _RelativeRanges(tuple(starts), tuple(buckets))
 
 
-def _same_device(what, device, *ts):
-    for t in ts:
-        if t is not None:
-            assert t.is_cuda, "rgd_triton_amd operators run on the GPU only"
-            assert t.device == device, f"{what}: tensors on {t.device} and {device}"
+# The functions below are called once per token, or between short kernels, where their host time is what a user waits for: tensor
+# attributes are read once, descriptors are packed bytes, the stream is asked for as a number.
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_desc4 = _hip.desc4
 
 
-def _on_device(device):
-    """Kernels are launched on the tensors' device, whichever is current."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, kernel_cache):
+    wstride = weight.stride()
+    device = weight.device
+    if not _seen(kernel_cache, "fwd", kernel_cache and (weight.shape, wstride, weight.dtype, device, seqlen_q, seqlen_k, q_offset, dtype, ranges)):
+        assert weight.is_cuda, "rgd_triton_amd operators run on the GPU only"
+        assert weight.dtype in _FLOATS and dtype in _FLOATS, "Only support fp16, bf16, and fp32"
+        assert weight.ndim == 2 and ranges.most < weight.shape[0], f"{weight.shape=}"
+        assert seqlen_q >= 0 and seqlen_k >= 0, f"{seqlen_q=}, {seqlen_k=}"
+    index = device.index
+    if index != _current_device():  # kernels are launched on the tensors' device, whichever is current
+        with torch.cuda.device(index):
+            return _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, None)
+    num_buckets, nheads = weight.shape
+    bias = torch.empty((1, nheads, seqlen_q, seqlen_k), dtype=dtype, device=device)
+    rc = _hip.lib().rgd_rel_bias_fwd(nheads, seqlen_q, seqlen_k, weight.data_ptr(), wstride[0], num_buckets,
+                                     _hip.dtype_code(weight.dtype), ranges.n, ranges.c_starts, ranges.c_buckets, q_offset,
+                                     _desc4(bias.data_ptr(), 0, seqlen_q * seqlen_k, seqlen_k), _hip.dtype_code(dtype),
+                                     _raw_stream(index))
+    if rc:
+        _hip.check(rc, "rgd_rel_bias_fwd")
+    return bias
+
+
+def _relative_bias_grad(dbias, num_buckets, nheads, seqlen_q, seqlen_k, ranges, q_offset, wdtype):
+    stride = dbias.stride()
+    if stride[3] != 1:
+        dbias = dbias.contiguous()
+        stride = dbias.stride()
+    device = dbias.device
+    index = device.index
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return _relative_bias_grad(dbias, num_buckets, nheads, seqlen_q, seqlen_k, ranges, q_offset, wdtype)
+    dw = torch.empty((num_buckets, nheads), dtype=wdtype, device=device)
+    lib = _hip.lib()
+    nbytes = lib.rgd_rel_bias_bwd_workspace(nheads, seqlen_q, seqlen_k, num_buckets)
+    ws = _hip.workspace(device, nbytes)
+    rc = lib.rgd_rel_bias_bwd(nheads, seqlen_q, seqlen_k, _desc4(dbias.data_ptr(), 0, stride[1], stride[2]),
+                              _hip.dtype_code(dbias.dtype), ranges.n, ranges.c_starts, ranges.c_buckets, q_offset, dw.data_ptr(),
+                              nheads, num_buckets, _hip.dtype_code(wdtype), ws.data_ptr(), nbytes, _raw_stream(index))
+    if rc:
+        _hip.check(rc, "rgd_rel_bias_bwd")
+    return dw
 
 
 class Relative_Bias_Func(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, seqlen_q, seqlen_k, ranges, q_offset=0, dtype=None, kernel_cache=None):
-        dtype = dtype or weight.dtype
-        (weight,) = _lastdim_contig(weight)
-        if not _seen(kernel_cache, "fwd", _sig(weight) + (seqlen_q, seqlen_k, q_offset, dtype, ranges, weight.device)):
-            assert weight.is_cuda, "rgd_triton_amd operators run on the GPU only"
-            assert weight.dtype in _FLOATS and dtype in _FLOATS, "Only support fp16, bf16, and fp32"
-            assert weight.ndim == 2 and max(ranges.buckets) < weight.shape[0], f"{weight.shape=}"
-            assert seqlen_q >= 0 and seqlen_k >= 0, f"{seqlen_q=}, {seqlen_k=}"
-        num_buckets, nheads = weight.shape
-        bias = torch.empty((1, nheads, seqlen_q, seqlen_k), dtype=dtype, device=weight.device)
-        lib = _hip.lib()
-        with _on_device(weight.device):
-            _hip.check(lib.rgd_rel_bias_fwd(nheads, seqlen_q, seqlen_k, weight.data_ptr(), weight.stride(0), num_buckets,
-                                            _hip.dtype_code(weight.dtype), ranges.n, ranges.c_starts, ranges.c_buckets, q_offset,
-                                            t4(bias, True), _hip.dtype_code(dtype), _hip.stream_ptr(weight.device)),
-                       "rgd_rel_bias_fwd")
+    def forward(ctx, weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, kernel_cache):
+        ctx.args = (weight.shape[0], weight.shape[1], seqlen_q, seqlen_k, ranges, q_offset, weight.dtype)
         ctx.kernel_cache = kernel_cache
-        ctx.args = (num_buckets, nheads, seqlen_q, seqlen_k, ranges, q_offset, weight.dtype)
-        return bias
+        return _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, kernel_cache)
 
     @staticmethod
     def backward(ctx, dbias):
         _no_capture("Relative_Bias_Func.backward")
-        num_buckets, nheads, seqlen_q, seqlen_k, ranges, q_offset, wdtype = ctx.args
-        (dbias,) = _lastdim_contig(dbias)
-        _seen(ctx.kernel_cache, "bwd", _sig(dbias))
-        dw = torch.empty((num_buckets, nheads), dtype=wdtype, device=dbias.device)
-        lib = _hip.lib()
-        nbytes = lib.rgd_rel_bias_bwd_workspace(nheads, seqlen_q, seqlen_k, num_buckets)
-        ws = _hip.workspace(dbias.device, nbytes)
-        with _on_device(dbias.device):
-            _hip.check(lib.rgd_rel_bias_bwd(nheads, seqlen_q, seqlen_k, t4(dbias, True), _hip.dtype_code(dbias.dtype), ranges.n,
-                                            ranges.c_starts, ranges.c_buckets, q_offset, dw.data_ptr(), nheads, num_buckets,
-                                            _hip.dtype_code(wdtype), ws.data_ptr(), nbytes, _hip.stream_ptr(dbias.device)),
-                       "rgd_rel_bias_bwd")
-        return dw, None, None, None, None, None, None
+        if ctx.kernel_cache is not None:
+            _seen(ctx.kernel_cache, "bwd", _sig(dbias))
+        return _relative_bias_grad(dbias, *ctx.args), None, None, None, None, None, None
 
 
 def relative_position_bias_fn(weight, seqlen_q, seqlen_k, max_distance=128, bidirectional=True, q_offset=0, dtype=None,
@@ -818,8 +832,12 @@ def relative_position_bias_fn(weight, seqlen_q, seqlen_k, max_distance=128, bidi
     bias[0, h, i, j] = weight[bucket of key j for query i + q_offset, h], weight (num_buckets, nheads); the buckets are
     relative_ranges'.  dtype: of the bias (the weight's by default; attention takes its own tensors' or fp32).  The
     gradient of the weight is summed in fp32 and rounded once."""
-    return Relative_Bias_Func.apply(weight, seqlen_q, seqlen_k, relative_ranges(weight.shape[0], max_distance, bool(bidirectional)),
-                                    q_offset, dtype, kernel_cache)
+    if weight.stride(-1) != 1:
+        weight = weight.contiguous()
+    ranges = relative_ranges(weight.shape[0], max_distance, bool(bidirectional))
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return Relative_Bias_Func.apply(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype or weight.dtype, kernel_cache)
+    return _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype or weight.dtype, kernel_cache)
 
 
 # ----------------------------------------------------------------------------------------------
@@ -828,20 +846,22 @@ def relative_position_bias_fn(weight, seqlen_q, seqlen_k, max_distance=128, bidi
 
 
 def _no_grad(what, *ts):
-    assert not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)), \
-        f"{what} is for serving and has no gradient: call it under torch.no_grad()"
+    for t in ts:
+        assert t is None or not t.requires_grad, f"{what} is for serving and has no gradient: call it under torch.no_grad()"
 
 
 def _check_cache(what, k_cache, v_cache, page_table, lens, batch, dtype, head_dim):
-    assert k_cache.ndim == 4 and k_cache.shape == v_cache.shape, f"{k_cache.shape=}, {v_cache.shape=}"
+    shape = k_cache.shape
+    assert len(shape) == 4 and shape == v_cache.shape, f"{k_cache.shape=}, {v_cache.shape=}"
     assert k_cache.stride(-1) == v_cache.stride(-1) == 1, f"{what}: the caches need unit-stride head dims"
     assert k_cache.dtype == v_cache.dtype == dtype, f"All tensors must have the same type {dtype=}, {k_cache.dtype=}, {v_cache.dtype=}"
     assert dtype in (torch.float16, torch.bfloat16), "Only support fp16 and bf16"
-    assert k_cache.shape[3] == head_dim <= 128, f"{what} only supports head dimensions up to 128, the cache's the same: {head_dim=}"
-    assert k_cache.shape[1] >= 1, f"{k_cache.shape=}: page size must be positive"
-    assert page_table.dtype == torch.int32 and page_table.ndim == 2 and page_table.shape[0] == batch, \
+    assert shape[3] == head_dim <= 128, f"{what} only supports head dimensions up to 128, the cache's the same: {head_dim=}"
+    assert shape[1] >= 1, f"{k_cache.shape=}: page size must be positive"
+    table = page_table.shape
+    assert page_table.dtype == torch.int32 and len(table) == 2 and table[0] == batch, \
         f"page_table is (batch, pages) int32: {page_table.dtype}, {page_table.shape}"
-    assert page_table.shape[1] <= 1 or page_table.stride(1) == 1, "page_table rows need unit stride"
+    assert table[1] <= 1 or page_table.stride(1) == 1, "page_table rows need unit stride"
     _check_lens(lens, batch)
 
 
@@ -850,9 +870,11 @@ def _check_lens(lens, batch):
         f"lengths are (batch,) int32, contiguous: {lens.dtype}, {lens.shape}"
 
 
-def _cache4(t):
-    # (num_pages, page_size, H, D) -> (page, head, slot) strides
-    return _hip.Tensor4(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1))
+def _check_device(what, index, *ts):
+    """index: get_device() of the operator's first tensor, -1 for one that is not on a GPU"""
+    assert index >= 0, "rgd_triton_amd operators run on the GPU only"
+    for t in ts:
+        assert t is None or t.get_device() == index, f"{what}: a tensor on {t.device}, another on cuda:{index}"
 
 
 def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens=None, seq_cutoff=None,
@@ -872,43 +894,56 @@ def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_tabl
     query, key, value = _lastdim_contig(query, key, value)
     if pos_emb is not None:
         (pos_emb,) = _lastdim_contig(_table_for(pos_emb, query))
-    _no_grad(what, query, key, value, pos_emb, k_cache, v_cache)
+    if torch.is_grad_enabled():
+        _no_grad(what, query, key, value, pos_emb, k_cache, v_cache)
     head, tok = (1, 2) if heads_second else (2, 1)
-    sig = _sig(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens)
-    if not _seen(kernel_cache, "fwd", sig + (bool(heads_second), query.device)):
-        assert query.ndim == key.ndim == value.ndim == 4
-        assert query.dtype == key.dtype == value.dtype, "All tensors must have the same type"
-        batch, T, D = query.shape[0], query.shape[tok], query.shape[3]
-        assert key.shape == value.shape and (key.shape[0], key.shape[tok], key.shape[3]) == (batch, T, D), \
+    shape, kshape, cache = query.shape, key.shape, k_cache.shape
+    index = query.get_device()
+    dtype = query.dtype
+    if not _seen(kernel_cache, "fwd", kernel_cache and _sig(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens) +
+                 (bool(heads_second), index)):
+        assert len(shape) == len(kshape) == 4
+        assert dtype == key.dtype == value.dtype, "All tensors must have the same type"
+        assert kshape == value.shape and kshape[0] == shape[0] and kshape[tok] == shape[tok] and kshape[3] == shape[3], \
             f"{query.shape=}, {key.shape=}, {value.shape=}"
-        _check_cache(what, k_cache, v_cache, page_table, cache_lens, batch, query.dtype, D)
-        assert k_cache.shape[2] == key.shape[head], f"{k_cache.shape=}, {key.shape=}"
+        _check_cache(what, k_cache, v_cache, page_table, cache_lens, shape[0], dtype, shape[3])
+        assert cache[2] == kshape[head], f"{k_cache.shape=}, {key.shape=}"
         if new_lens is not None:
-            _check_lens(new_lens, batch)
+            _check_lens(new_lens, shape[0])
         if pos_emb is not None:
             assert pos_emb.ndim == 3 and pos_emb.shape[0] == 2 and pos_emb.dtype in _FLOATS, f"{pos_emb.shape=}"
-            assert pos_emb.shape[2] <= D and pos_emb.shape[2] % 2 == 0, f"{pos_emb.shape=}: an even rotary dim, at most {D=}"
-            assert pos_emb.shape[1] >= page_table.shape[1] * k_cache.shape[1], \
-                f"{pos_emb.shape=}: a row for every position of {page_table.shape[1]} pages of {k_cache.shape[1]}"
-        _same_device(what, query.device, query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens)
-    B, Hq, T, D = query.shape[0], query.shape[head], query.shape[tok], query.shape[3]
-    num_pages, page_size, Hkv, _ = k_cache.shape
+            assert pos_emb.shape[2] <= shape[3] and pos_emb.shape[2] % 2 == 0, f"{pos_emb.shape=}: an even rotary dim, at most {shape[3]}"
+            assert pos_emb.shape[1] >= page_table.shape[1] * cache[1], \
+                f"{pos_emb.shape=}: a row for every position of {page_table.shape[1]} pages of {cache[1]}"
+        _check_device(what, index, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens, seq_cutoff,
+                                        heads_second, norm_eps)
     if pos_emb is None:
         pe = (None, 0, 0, 0, 0, _hip.RGD_F32)
     else:
-        pe = (pos_emb.data_ptr(), pos_emb.shape[1], pos_emb.shape[2], pos_emb.stride(0), pos_emb.stride(1), _hip.dtype_code(pos_emb.dtype))
+        _, P, R = pos_emb.shape
+        ss, sn, _ = pos_emb.stride()
+        pe = (pos_emb.data_ptr(), P, R, ss, sn, _hip.dtype_code(pos_emb.dtype))
     cq, ck = _cutoffs(seq_cutoff, 2**31 - 1, 2**31 - 1)
     qo = torch.empty_like(query)
-    lib = _hip.lib()
-    with _on_device(query.device):
-        _hip.check(lib.rgd_rope_cache_append(
-            B, T, Hq, Hkv, D, t4(query, heads_second), t4(key, heads_second), t4(value, heads_second), t4(qo, heads_second),
-            _cache4(k_cache), _cache4(v_cache), num_pages, page_size, page_table.data_ptr(), page_table.shape[1],
-            page_table.stride(0), cache_lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(), *pe, cq, ck,
-            int(norm_eps is not None), float(norm_eps or 0.0), _hip.dtype_code(query.dtype), _hip.stream_ptr(query.device)),
-            "rgd_rope_cache_append")
+    sq, sk, sv, so, ck_s, cv_s = query.stride(), key.stride(), value.stride(), qo.stride(), k_cache.stride(), v_cache.stride()
+    rc = _hip.lib().rgd_rope_cache_append(
+        shape[0], shape[tok], shape[head], kshape[head], shape[3],
+        _desc4(query.data_ptr(), sq[0], sq[head], sq[tok]), _desc4(key.data_ptr(), sk[0], sk[head], sk[tok]),
+        _desc4(value.data_ptr(), sv[0], sv[head], sv[tok]), _desc4(qo.data_ptr(), so[0], so[head], so[tok]),
+        _desc4(k_cache.data_ptr(), ck_s[0], ck_s[2], ck_s[1]), _desc4(v_cache.data_ptr(), cv_s[0], cv_s[2], cv_s[1]),
+        cache[0], cache[1], page_table.data_ptr(), page_table.shape[1], page_table.stride(0), cache_lens.data_ptr(),
+        None if new_lens is None else new_lens.data_ptr(), *pe, cq, ck, norm_eps is not None, norm_eps or 0.0,
+        _hip.dtype_code(dtype), _raw_stream(index))
+    if rc:
+        _hip.check(rc, "rgd_rope_cache_append")
     torch.autograd.graph.increment_version((k_cache, v_cache))
     return qo
+
+
+_NO_BIAS = (None, 0, 0, _hip.RGD_F32, 0, None, None)
 
 
 def paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight=None, max_distance=128, bidirectional=True,
@@ -921,32 +956,45 @@ def paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight
     seq_lens[b] - 1.  Returns o (B, 1, Hq, D), with return_lse also the logsumexp (B, Hq) in fp32.  A sequence without keys gives
     o = 0, lse = -inf.  Keys on a page number outside the cache are not seen; lengths beyond the page table end there."""
     what = "paged_decode_attn"
-    q, rel_weight = _lastdim_contig(q, rel_weight)
-    _no_grad(what, q, k_cache, v_cache, rel_weight)
-    if not _seen(kernel_cache, "fwd", _sig(q, k_cache, v_cache, page_table, seq_lens, rel_weight) + (q.device,)):
-        assert q.ndim == 4 and q.shape[1] == 1, f"{q.shape=}: one new token per sequence"
-        _check_cache(what, k_cache, v_cache, page_table, seq_lens, q.shape[0], q.dtype, q.shape[3])
-        assert k_cache.shape[2] >= 1 and q.shape[2] % k_cache.shape[2] == 0, f"{q.shape=}, {k_cache.shape=}: query heads in groups"
+    sq = q.stride()
+    if sq[-1] != 1:
+        q = q.contiguous()
+        sq = q.stride()
+    if rel_weight is not None and rel_weight.stride(-1) != 1:
+        rel_weight = rel_weight.contiguous()
+    if torch.is_grad_enabled():
+        _no_grad(what, q, k_cache, v_cache, rel_weight)
+    shape, cache = q.shape, k_cache.shape
+    index = q.get_device()
+    dtype = q.dtype
+    if not _seen(kernel_cache, "fwd", kernel_cache and _sig(q, k_cache, v_cache, page_table, seq_lens, rel_weight) + (index,)):
+        assert len(shape) == 4 and shape[1] == 1, f"{q.shape=}: one new token per sequence"
+        _check_cache(what, k_cache, v_cache, page_table, seq_lens, shape[0], dtype, shape[3])
+        assert cache[2] >= 1 and shape[2] % cache[2] == 0, f"{q.shape=}, {k_cache.shape=}: query heads in groups"
         if rel_weight is not None:
-            assert rel_weight.ndim == 2 and rel_weight.shape[1] == q.shape[2] and rel_weight.dtype in _FLOATS, f"{rel_weight.shape=}"
-        _same_device(what, q.device, q, k_cache, v_cache, page_table, seq_lens, rel_weight)
-    B, _, Hq, D = q.shape
-    num_pages, page_size, Hkv, _ = k_cache.shape
-    softmax_scale = softmax_scale or 1.0 / math.sqrt(D)
-    rel = (None, 0, 0, _hip.RGD_F32, 0, None, None)
+            assert rel_weight.ndim == 2 and rel_weight.shape[1] == shape[2] and rel_weight.dtype in _FLOATS, f"{rel_weight.shape=}"
+        _check_device(what, index, k_cache, v_cache, page_table, seq_lens, rel_weight)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight, max_distance, bidirectional,
+                                          softmax_scale, return_lse)
+    B, _, Hq, D = shape
+    rel = _NO_BIAS
     if rel_weight is not None:
         r = relative_ranges(rel_weight.shape[0], max_distance, bool(bidirectional))
         rel = (rel_weight.data_ptr(), rel_weight.stride(0), rel_weight.shape[0], _hip.dtype_code(rel_weight.dtype), r.n, r.c_starts,
                r.c_buckets)
-    o = torch.empty((B, 1, Hq, D), dtype=q.dtype, device=q.device)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     lib = _hip.lib()
-    nbytes = lib.rgd_paged_decode_workspace(B, Hq, Hkv, D)
+    nbytes = lib.rgd_paged_decode_workspace(B, Hq, cache[2], D)
     ws = _hip.workspace(q.device, nbytes)
-    with _on_device(q.device):
-        _hip.check(lib.rgd_paged_decode(
-            B, Hq, Hkv, D, t4(q, False), _cache4(k_cache), _cache4(v_cache), num_pages, page_size, page_table.data_ptr(),
-            page_table.shape[1], page_table.stride(0), seq_lens.data_ptr(), *rel, t4(o, False),
-            None if lse is None else lse.data_ptr(), _hip.dtype_code(q.dtype), float(softmax_scale), ws.data_ptr(), nbytes,
-            _hip.stream_ptr(q.device)), "rgd_paged_decode")
+    ck_s, cv_s = k_cache.stride(), v_cache.stride()
+    rc = lib.rgd_paged_decode(
+        B, Hq, cache[2], D, _desc4(q.data_ptr(), sq[0], sq[2], sq[1]), _desc4(k_cache.data_ptr(), ck_s[0], ck_s[2], ck_s[1]),
+        _desc4(v_cache.data_ptr(), cv_s[0], cv_s[2], cv_s[1]), cache[0], cache[1], page_table.data_ptr(), page_table.shape[1],
+        page_table.stride(0), seq_lens.data_ptr(), *rel, _desc4(o.data_ptr(), Hq * D, D, 0), None if lse is None else lse.data_ptr(),
+        _hip.dtype_code(dtype), softmax_scale or 1.0 / math.sqrt(D), ws.data_ptr(), nbytes, _raw_stream(index))
+    if rc:
+        _hip.check(rc, "rgd_paged_decode")
     return (o, lse) if return_lse else o

@@ -12,7 +12,7 @@ from serving_helpers import gen, randn, rotary, serving_oracle
 
 from rgd_triton_amd import _hip
 
-T4 = _hip.Tensor4(0x1000, 4096, 64, 64)
+T4 = _hip.desc4(0x1000, 4096, 64, 64)
 BUF = ctypes.c_void_p(0x1000)
 
 
