@@ -4,15 +4,14 @@
 //
 // Bound by memory: every cached key and value is read once, 4 D bytes per token and key head, for 4 D group operations.
 //
-// Work.  A unit is (sequence, key head, 16 of the key head's query heads); its keys are cut into tiles of 128.  The tiles of all
-// units, in one row, are dealt to the workgroups in equal runs: every workgroup finds its run from the lengths on the GPU, so
-// the host need not know them, one long sequence fills the chip like many short ones, and a ragged batch leaves no workgroup
+// Work.  A unit is (sequence, key head, 16 of the key head's query heads); its keys are cut into tiles of 32.  The tiles of all
+// units, in one row, are dealt to the wavefronts in equal runs: every wavefront finds its run from the lengths on the GPU, so
+// the host need not know them, one long sequence fills the chip like many short ones, and a ragged batch leaves no wavefront
 // with more than a tile over the others.  A run that holds a whole unit writes its output; pieces of a unit that several
-// workgroups share leave partial results in the workspace (at most two per workgroup: one unit begun earlier, one not ended),
+// wavefronts share leave partial results in the workspace (at most two per wavefront: one unit begun earlier, one not ended),
 // which the merge launch joins in order.
 //
-// A step.  Each of the four wavefronts walks every fourth 32 keys on its own, without LDS or barriers, operands straight
-// from memory to registers (v_mfma_f32_16x16x32: A lane l holds row l % 16, k = 8 (l / 16) .. + 7; C lane l holds column l % 16,
+// A step.  A wavefront (a workgroup of its own) takes 32 keys at a time, without LDS or barriers, operands straight from memory to registers (v_mfma_f32_16x16x32: A lane l holds row l % 16, k = 8 (l / 16) .. + 7; C lane l holds column l % 16,
 // rows 4 (l / 16) + 0..3):
 //   S^T = K Q^T, two products of 16 keys.  MFMA row i of product a is key 8 (i / 4) + 4 a + i % 4, so that lane group g = l / 16 ends
 //   up with the logits of keys 8 g .. 8 g + 7 of query head l % 16: the layout P^T has to have as the second product's B operand.
@@ -29,7 +28,7 @@
 #include <type_traits>
 
 constexpr int DEC_MAX_RANGES = 256;
-constexpr int DEC_TILE = 128;  // keys of a scheduling tile: 4 wavefronts x 32
+constexpr int DEC_TILE = 32;  // keys of a step
 
 struct DecodeParams {
     const void* q;
@@ -46,9 +45,10 @@ struct DecodeParams {
     int D, num_pages;
     FastDiv div_page;
     float scale;
-    int2* plan;        // per unit of the batch: workgroups its first and last piece are in
-    float* part;       // two slots per workgroup: O [rows][DP], then m [16], l [16]
+    int2* plan;        // per unit of the batch: wavefronts its first and last piece are in
+    float* part;       // two slots per wavefront: O [rows][DP], then m [16], l [16]
     int part_rows;     // query heads of a slot
+    int least;         // tiles of a run at least
 };
 
 struct DecodeBias {  // relative bias: weight (buckets, Hq), ranges of the distance and their buckets
@@ -75,6 +75,22 @@ template <> struct Mfma16<f16_t> {
 template <int N> __device__ __forceinline__ void load_dwords(const char* p, uint32_t (&out)[N]) {
     __builtin_memcpy(out, p, 4 * N);
 }
+#ifndef DEC_NT
+#define DEC_NT 1
+#endif
+template <int N> __device__ __forceinline__ void stream_dwords(const char* p, uint32_t (&out)[N]) {
+    if constexpr (!DEC_NT) { load_dwords<N>(p, out); return; }
+    if constexpr (N == 1) {
+        typedef uint32_t V __attribute__((aligned(2)));
+        out[0] = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+    } else {
+        typedef uint32_t V0 __attribute__((ext_vector_type(N)));
+        typedef V0 V __attribute__((aligned(2)));
+        const V0 v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = v[i];
+    }
+}
 
 // a value that is the same in all lanes, for the scalar unit
 __device__ __forceinline__ int64_t uniform64(int64_t v) {
@@ -93,167 +109,117 @@ constexpr float DEC_LAZY = 5.5f;
 // What is left is at most (2^-7 + 2^-8) p, its own rounding 2^-14.4 p.
 constexpr float DEC_HIGH = 1.0f - 1.0f / 128;
 
-struct DecodePiece {
-    int b, unit, len, t0, t1;  // keys [t0, t1)
-};
-
 // NC: 32-channel chunks of the head dim (DP = 32 NC).  PAGE8: the page size is a multiple of 8, so the 8 keys of a lane group
-// stand in one page (one lookup instead of 8).  SMALL: D < 8, rows are read element by element.
+// stand in one page and a lane needs two page numbers; otherwise the lanes look up the 32 keys' pages together and pass
+// the row addresses around.  SMALL: D < 8, rows are read element by element.
 template <typename T, int NC, bool PAGE8, bool SMALL, bool BIAS>
-__global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p,
-                                                           const std::conditional_t<BIAS, DecodeBias, DecodeNoBias> rel) {
-    constexpr int DP = 32 * NC, VE = DP / 16, VW = VE / 2, OSTRIDE = DP + 4;
-    __shared__ float s_o[4][16][OSTRIDE];
-    __shared__ float s_m[4][16], s_l[4][16];
-    __shared__ int s_scan[256];
-    __shared__ int64_t s_at[4];
+__global__ __launch_bounds__(64) void paged_decode_kernel(const DecodeParams p,
+                                                          const std::conditional_t<BIAS, DecodeBias, DecodeNoBias> rel) {
+    constexpr int DP = 32 * NC, VE = DP / 16, VW = VE / 2;
     __shared__ int s_start[BIAS ? DEC_MAX_RANGES : 1];
     __shared__ float s_w[BIAS ? DEC_MAX_RANGES : 1][16];
 
-    const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = threadIdx.x;
     const int n16 = lane & 15, g = lane >> 4;
     const int D = p.D;
     auto length = [&](int b) {
         const int n = p.seq_lens[b];
         return n < 0 ? 0 : (n < p.capacity ? n : p.capacity);
     };
-    auto tiles_of = [](int len) { return len > 0 ? (len + DEC_TILE - 1) / DEC_TILE : 1; };
+    auto tiles_of = [](int len) { return len > 0 ? (int)(((uint32_t)len + DEC_TILE - 1) / DEC_TILE) : 1; };
 
-    // ---- this workgroup's run of tiles
-    int64_t total = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 256) {
-        int n = b0 + tid < p.B ? tiles_of(length(b0 + tid)) : 0;
+    // ---- this wavefront's run of tiles [x, x_end) and the sequence it begins in
+    auto scan = [&](uint32_t n) {  // inclusive sum over the lanes (64 sequences of at most 2^26 tiles)
 #pragma unroll
-        for (int m = 1; m < 64; m <<= 1) n += __shfl_xor(n, m, 64);
-        if (lane == 0) s_scan[wave] = n;
-        __syncthreads();
-        total += uniform64((int64_t)s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3]);
-        __syncthreads();
-    }
+        for (int m = 1; m < 64; m <<= 1) {
+            const uint32_t up = __shfl_up(n, m, 64);
+            if (lane >= m) n += up;
+        }
+        return n;
+    };
+    auto last_of = [](uint32_t n) { return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)n, 63); };
+    uint32_t mine = lane < p.B ? tiles_of(length(lane)) : 0;  // tiles of sequence b0 + lane
+    uint32_t incl = scan(mine);
+    int64_t total = last_of(incl);
+    for (int b0 = 64; b0 < p.B; b0 += 64) total += last_of(scan(b0 + lane < p.B ? tiles_of(length(b0 + lane)) : 0));
     total *= p.units;
-    const int64_t share = (total + gridDim.x - 1) / gridDim.x;
+    const int64_t even = total <= INT32_MAX ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x) : (total + gridDim.x - 1) / gridDim.x;
+    const int64_t share = max(even, (int64_t)p.least);
     int64_t x = share * blockIdx.x;
     const int64_t x_end = min(total, x + share);
     if (x >= x_end) return;
-
-    // ---- the sequence, unit and tile it begins with
     int b = 0;
     int64_t base = 0;  // first tile of sequence b
-    for (int b0 = 0;; b0 += 256) {
-        int n = b0 + tid < p.B ? tiles_of(length(b0 + tid)) : 0;
-        int incl = n;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int up = __shfl_up(incl, m, 64);
-            if (lane >= m) incl += up;
-        }
-        if (lane == 63) s_scan[wave] = incl;
-        if (tid == 0) s_at[0] = -1;
-        __syncthreads();
-        int64_t before = 0, all = 0;  // (64 sequences' tiles fit 31 bits, 256 may not)
-        for (int w = 0; w < 4; ++w) {
-            before += w < wave ? s_scan[w] : 0;
-            all += s_scan[w];
-        }
-        const int64_t end = base + (before + incl) * p.units, begin = end - (int64_t)n * p.units;
-        if (x >= begin && x < end) {
-            s_at[0] = b0 + tid;
-            s_at[1] = begin;
-        }
-        __syncthreads();
-        if (s_at[0] >= 0) {
-            b = __builtin_amdgcn_readfirstlane((int)s_at[0]);
-            base = uniform64(s_at[1]);
+    for (int b0 = 0;;) {
+        const uint64_t behind = __ballot(base + (int64_t)incl * p.units > x);
+        if (behind) {
+            const int at = __builtin_ctzll(behind);
+            b = b0 + at;
+            base += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), at) * p.units;
             break;
         }
-        base += uniform64(all) * p.units;
-        __syncthreads();
+        base += last_of(incl) * p.units;
+        b0 += 64;
+        mine = b0 + lane < p.B ? tiles_of(length(b0 + lane)) : 0;
+        incl = scan(mine);
     }
 
     while (x < x_end) {
         const int len = __builtin_amdgcn_readfirstlane(length(b));
         const int ntiles = tiles_of(len);
         const int64_t in_seq = x - base;
-        const int unit = (int)(in_seq / ntiles), tile0 = (int)(in_seq - (int64_t)unit * ntiles);
+        const int unit = in_seq <= INT32_MAX ? (int)((uint32_t)in_seq / (uint32_t)ntiles) : (int)(in_seq / ntiles);
+        const int tile0 = (int)(in_seq - (int64_t)unit * ntiles);
         const int tile1 = (int)min((int64_t)ntiles, tile0 + (x_end - x));
-        const int t_end = min(len, tile1 * DEC_TILE);
         const int hk = unit / p.head_tiles, head0 = hk * p.group + (unit - hk * p.head_tiles) * 16;
         const int heads = min(16, (hk + 1) * p.group - head0);
-
-        if constexpr (BIAS) {
-            __syncthreads();
-            for (int i = tid; i < rel.n_ranges * 16; i += 256) {
-                const int r = i >> 4, h = i & 15;
-                float wv = 0.f;
-                if (h < heads) {
-                    const int64_t at = rel.bucket[r] * rel.w_stride + head0 + h;
-                    wv = rel.w_dtype == RGD_F32 ? static_cast<const float*>(rel.w)[at]
-                         : rel.w_dtype == RGD_F16 ? to_f32(static_cast<const f16_t*>(rel.w)[at]) : to_f32(static_cast<const bf16_t*>(rel.w)[at]);
-                }
-                s_w[r][h] = wv;
-                if (h == 0) s_start[r] = r == 0 ? INT32_MIN : rel.start[r];
-            }
-            __syncthreads();
-        }
-
-        // ---- query operand: B operand of S^T = K Q^T, head n16, channels of chunk 4 c + g
-        u32x4 qf[NC];
-        u32x4 kmask;  // channels of the last chunk that are not an earlier chunk's (all ones where the row is long enough)
-        int kstart[NC];
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int ci = (4 * c + g) * 8;
-            kstart[c] = SMALL ? 0 : min(ci, D - 8);
-            Pack16 raw, keep;
-            raw.v = u32x4{0, 0, 0, 0};
-            const T* qrow = static_cast<const T*>(p.q) + b * p.sq[0] + (int64_t)(head0 + min(n16, heads - 1)) * p.sq[1];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool mine = SMALL ? ci + e < D : kstart[c] + e >= ci;
-                keep.h[e] = mine ? 0xFFFF : 0;
-                const int d = SMALL ? min(e, D - 1) : kstart[c] + e;
-                const uint16_t qe = reinterpret_cast<const uint16_t*>(qrow)[d];
-                raw.h[e] = mine && n16 < heads ? qe : 0;
-            }
-            qf[c] = raw.v;
-            kmask = keep.v;
-        }
-        const int vstart = SMALL ? n16 * VE : min(n16 * VE, D - VE);
-
-        f32x4 acc[VE];
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float ref = -INFINITY, l = 0.f;
 
         const T* kbase = static_cast<const T*>(p.k) + hk * p.sk[1];
         const T* vbase = static_cast<const T*>(p.v) + hk * p.sv[1];
         const int32_t* table = p.page_table + b * p.table_stride;
-        constexpr int NK = PAGE8 ? 1 : 2, NV = PAGE8 ? 1 : 8;
-        int ek[NK], ev[NV];  // page numbers of the next step's keys and values
+
+        u32x4 qf[NC];
+        u32x4 kmask;  // channels of the last chunk that are not an earlier chunk's (all ones where the row is long enough)
+        int kstart[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) kstart[c] = SMALL ? 0 : min((4 * c + g) * 8, D - 8);
+        const int vstart = SMALL ? n16 * VE : min(n16 * VE, D - VE);
+
         u32x4 kf[2][NC];
         uint32_t vr[8][VW];
-        bool v_ok[NV], v_ok_next[NV];
+        // Page numbers are looked up two steps ahead and turned into row addresses one step ahead: loads return in order, so a
+        // lookup behind a step's loads would hold up the next step's until those are there.
+        int e0 = 0, e1 = 0;                // PAGE8: page numbers of the lane's keys and values; else e0: of key t + lane % 32
+        int64_t koff = 0, voff = 0;        // row offsets: PAGE8: of the lane's first key and value; else: of key t + lane % 32
+        uint64_t ok_cur = 0, ok_next = 0;  // ballot of "the page exists": PAGE8: of the lane's values; else: bit i for key t + i
 
-        // token a lane's lookup i stands for (clamped to the sequence, so that only its own page numbers are read)
-        auto ktok = [&](int t, int i) {
-            return PAGE8 ? min(t + 8 * (n16 >> 2), (len - 1) & ~7) : min(t + 8 * (n16 >> 2) + 4 * i + (n16 & 3), len - 1);
+        auto lookup = [&](int t) __attribute__((always_inline)) {  // (clamped: only the sequence's own page numbers are read)
+            if constexpr (PAGE8) {
+                e0 = table[fast_div(min(t + 8 * (n16 >> 2), (len - 1) & ~7), p.div_page)];
+                e1 = table[fast_div(min(t + 8 * g, (len - 1) & ~7), p.div_page)];
+            } else {
+                e0 = table[fast_div(min(t + (lane & 31), len - 1), p.div_page)];
+            }
         };
-        auto vtok = [&](int t, int i) { return PAGE8 ? min(t + 8 * g, (len - 1) & ~7) : min(t + 8 * g + i, len - 1); };
-        auto lookup = [&](int t) {
-#pragma unroll
-            for (int i = 0; i < NK; ++i) ek[i] = table[fast_div(ktok(t, i), p.div_page)];
-#pragma unroll
-            for (int i = 0; i < NV; ++i) ev[i] = table[fast_div(vtok(t, i), p.div_page)];
+        auto locate = [&](int t) __attribute__((always_inline)) {
+            auto slot_of = [&](int tok) { return tok - (int)(fast_div(tok, p.div_page) * p.div_page.d); };
+            const bool ok0 = e0 >= 0 && e0 < p.num_pages;
+            if constexpr (PAGE8) {
+                const bool ok1 = e1 >= 0 && e1 < p.num_pages;
+                ok_next = __ballot(ok1);
+                koff = (ok0 ? e0 : 0) * p.sk[0] + (slot_of(min(t + 8 * (n16 >> 2), (len - 1) & ~7)) + (n16 & 3)) * p.sk[2];
+                voff = (ok1 ? e1 : 0) * p.sv[0] + slot_of(min(t + 8 * g, (len - 1) & ~7)) * p.sv[2];
+            } else {
+                const int slot = slot_of(min(t + (lane & 31), len - 1));
+                ok_next = __ballot(ok0);
+                koff = (ok0 ? e0 : 0) * p.sk[0] + slot * p.sk[2];
+                voff = (ok0 ? e0 : 0) * p.sv[0] + slot * p.sv[2];
+            }
         };
-        auto load_k = [&](int t) {
+        auto load_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
-                const int tok = ktok(t, a);
-                int slot = tok - (int)(fast_div(tok, p.div_page) * p.div_page.d);
-                if (PAGE8) slot += 4 * a + (n16 & 3);
-                const int e = ek[PAGE8 ? 0 : a];
-                const int page = e >= 0 && e < p.num_pages ? e : 0;
-                const T* row = kbase + page * p.sk[0] + slot * p.sk[2];
+                const T* row = kbase + (PAGE8 ? koff + 4 * a * p.sk[2] : __shfl(koff, 8 * (n16 >> 2) + 4 * a + (n16 & 3), 64));
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     if constexpr (SMALL) {
@@ -263,32 +229,53 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p,
                         kf[a][c] = r.v;
                     } else {
                         uint32_t r[4];
-                        load_dwords<4>(reinterpret_cast<const char*>(row + kstart[c]), r);
+                        stream_dwords<4>(reinterpret_cast<const char*>(row + kstart[c]), r);
                         kf[a][c] = u32x4{r[0], r[1], r[2], r[3]};
                     }
                 }
             }
         };
-        auto load_v = [&](int t) {
+        auto load_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int tok = vtok(t, i);
-                int slot = tok - (int)(fast_div(tok, p.div_page) * p.div_page.d);
-                if (PAGE8) slot += i;
-                const int e = ev[PAGE8 ? 0 : i];
-                const bool ok = e >= 0 && e < p.num_pages;
-                if (!PAGE8 || i == 0) v_ok_next[PAGE8 ? 0 : i] = ok;
-                const int page = ok ? e : 0;
-                const T* row = vbase + page * p.sv[0] + slot * p.sv[2];
+                const T* row = vbase + (PAGE8 ? voff + i * p.sv[2] : __shfl(voff, 8 * g + i, 64));
                 if constexpr (SMALL) {
                     const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
                     vr[i][0] = r[min(vstart, D - 1)] | (uint32_t)r[min(vstart + 1, D - 1)] << 16;
                 } else {
-                    load_dwords<VW>(reinterpret_cast<const char*>(row + vstart), vr[i]);
+                    stream_dwords<VW>(reinterpret_cast<const char*>(row + vstart), vr[i]);
                 }
             }
         };
 
+        // ---- the first step's loads on their way, then what does not depend on them
+        const int t0 = tile0 * DEC_TILE;
+        if (len > 0) lookup(t0);
+        // query: B operand of S^T = K Q^T, head n16, channels of chunk 4 c + g
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int ci = (4 * c + g) * 8;
+            Pack16 raw, keep;
+            const T* qrow = static_cast<const T*>(p.q) + b * p.sq[0] + (int64_t)(head0 + min(n16, heads - 1)) * p.sq[1];
+            if constexpr (SMALL) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) raw.h[e] = reinterpret_cast<const uint16_t*>(qrow)[min(e, D - 1)];
+            } else {
+                load_dwords<4>(reinterpret_cast<const char*>(qrow + kstart[c]), raw.w);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) keep.h[e] = (SMALL ? ci + e < D : kstart[c] + e >= ci) ? 0xFFFF : 0;
+            raw.v = n16 < heads ? raw.v & keep.v : u32x4{0, 0, 0, 0};
+            qf[c] = raw.v;
+            kmask = keep.v;
+        }
+        f32x4 acc[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float ref = -INFINITY, l = 0.f;
+        const int hrow = min(n16, heads - 1);
+
+        // one step; prefetch: the next one's keys are loaded as soon as this one's are used
         auto step = [&](int t, bool prefetch) __attribute__((always_inline)) {
             f32x4 s[2];
 #pragma unroll
@@ -301,19 +288,20 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p,
                     s[a] = Mfma16<T>::run(kk, qf[c], s[a]);
                 }
             }
-            const bool ok0 = v_ok[0];
-            bool ok_all = ok0;
-#pragma unroll
-            for (int i = 1; i < NV; ++i) ok_all = ok_all && v_ok[i];
-            const bool whole = t + 32 <= len && __all(ok_all);
-            if (prefetch) load_k(t + DEC_TILE);
+            const bool whole = t + 32 <= len && (PAGE8 ? ok_cur == ~0ull : (uint32_t)ok_cur == ~0u);
+            const uint32_t ok8 = PAGE8 ? ((ok_cur >> lane) & 1 ? 0xFFu : 0u) : (uint32_t)ok_cur >> (8 * g);  // of the lane's 8 keys
+            if (prefetch) {
+                locate(t + DEC_TILE);
+                lookup(t + 2 * DEC_TILE);
+                load_k();
+            }
             float x8[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) x8[i] = s[i >> 2][i & 3] * p.scale;
             if constexpr (BIAS) {
                 const int d0 = t + 8 * g - (len - 1);
                 if (t + 31 - (len - 1) < s_start[min(1, rel.n_ranges - 1)]) {  // all in the first range
-                    const float wv = s_w[0][n16];
+                    const float wv = s_w[0][hrow];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x8[i] += wv;
                 } else {
@@ -326,14 +314,14 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p,
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         while (lo + 1 < rel.n_ranges && s_start[lo + 1] <= d0 + i) ++lo;
-                        x8[i] += s_w[lo][n16];
+                        x8[i] += s_w[lo][hrow];
                     }
                 }
             }
             if (!whole) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (!(t + 8 * g + i < len && v_ok[PAGE8 ? 0 : i])) x8[i] = -INFINITY;
+                    if (!(t + 8 * g + i < len && (ok8 >> i & 1))) x8[i] = -INFINITY;
             }
             float top = fmaxf(fmaxf(fmaxf(x8[0], x8[1]), fmaxf(x8[2], x8[3])), fmaxf(fmaxf(x8[4], x8[5]), fmaxf(x8[6], x8[7])));
             if (__any(top > ref + DEC_LAZY)) {
@@ -366,7 +354,7 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p,
             if (!whole) {  // what stands in slots of no key may be anything: 0 * NaN is NaN
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const bool in = t + 8 * g + i < len && v_ok[PAGE8 ? 0 : i];
+                    const bool in = t + 8 * g + i < len && (ok8 >> i & 1);
 #pragma unroll
                     for (int w = 0; w < VW; ++w) vr[i][w] = in ? vr[i][w] : 0u;
                 }
@@ -382,65 +370,76 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p,
             }
         };
 
-        int t = tile0 * DEC_TILE + 32 * wave;
-        if (t < t_end) {
-            lookup(t);
-            load_k(t);
-            load_v(t);
-            if (t + DEC_TILE < t_end) lookup(t + DEC_TILE);
-            for (; t + DEC_TILE < t_end; t += DEC_TILE) {
-#pragma unroll
-                for (int i = 0; i < NV; ++i) v_ok[i] = v_ok_next[i];
-                step(t, true);
-                load_v(t + DEC_TILE);
-                lookup(t + 2 * DEC_TILE);
+        if (len > 0) {
+            locate(t0);
+            lookup(t0 + DEC_TILE);
+            load_k();
+            __builtin_amdgcn_sched_barrier(0);  // (keys before values here as in the loop: waits count loads in order)
+            load_v();
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (BIAS) {  // the weight of the unit's heads, by range
+                const int hb = heads > 1 ? 32 - __builtin_clz(heads - 1) : 0;
+#pragma unroll 4
+                for (int i = lane; i < rel.n_ranges << hb; i += 64) {
+                    const int r = i >> hb, h = min(i - (r << hb), heads - 1);
+                    const int64_t at = rel.bucket[r] * rel.w_stride + head0 + h;
+                    s_w[r][h] = rel.w_dtype == RGD_F32 ? static_cast<const float*>(rel.w)[at]
+                                : rel.w_dtype == RGD_F16 ? to_f32(static_cast<const f16_t*>(rel.w)[at])
+                                                         : to_f32(static_cast<const bf16_t*>(rel.w)[at]);
+                    if (i == r << hb) s_start[r] = r == 0 ? INT32_MIN : rel.start[r];
+                }
+                __syncthreads();  // (one wavefront: orders its LDS accesses)
             }
-#pragma unroll
-            for (int i = 0; i < NV; ++i) v_ok[i] = v_ok_next[i];
-            step(t, false);
+            const int t_last = (tile1 - 1) * DEC_TILE;
+            for (int t = t0; t < t_last; t += DEC_TILE) {
+                ok_cur = ok_next;
+                step(t, true);
+                load_v();
+            }
+            ok_cur = ok_next;
+            step(t_last, false);
         }
 
-        // ---- join the wavefronts
+        // ---- the piece's result: lane holds channels VE m + e of head n16 for m = 4 g + r
         l += xor_lanes(l, 16);
         l += xor_lanes(l, 32);
-        __syncthreads();  // (the buffers' readers of the piece before are done)
-        if (g == 0) {
-            s_m[wave][n16] = ref;
-            s_l[wave][n16] = l;
+        const bool begins = tile0 == 0, ends = tile1 == ntiles;
+        if (begins && lane == 0) {
+            const int64_t last = base + (int64_t)unit * ntiles + ntiles - 1;
+            p.plan[(int64_t)b * p.units + unit] = make_int2((int)blockIdx.x, (int)(last <= INT32_MAX && share <= INT32_MAX ? (uint32_t)last / (uint32_t)share : last / share));
         }
         if (n16 < heads) {
+            if (begins && ends) {
+                const float inv = l == 0.f ? 0.f : 1.0f / l;
+                T* orow = static_cast<T*>(p.o) + b * p.so[0] + (int64_t)(head0 + n16) * p.so[1];
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+                for (int r = 0; r < 4; ++r) {
+                    const int first = (4 * g + r) * VE;
+                    T out[VE];
 #pragma unroll
-                for (int e = 0; e < VE; ++e) s_o[wave][n16][(4 * g + r) * VE + e] = acc[e][r];
-        }
-        __syncthreads();
-        const bool begins = tile0 == 0, ends = tile1 == ntiles;
-        const bool direct = begins && ends;
-        if (begins && tid == 0) {
-            const int64_t first = base + (int64_t)unit * ntiles;
-            p.plan[(int64_t)b * p.units + unit] = make_int2((int)blockIdx.x, (int)((first + ntiles - 1) / share));
-        }
-        float* slot = p.part + (int64_t)(2 * blockIdx.x + (begins ? 1 : 0)) * ((int64_t)p.part_rows * DP + 32);
-        for (int i = tid; i < heads * DP; i += 256) {
-            const int h = i / DP, at = i - h * DP;
-            const float m0 = s_m[0][h], m1 = s_m[1][h], m2 = s_m[2][h], m3 = s_m[3][h];
-            const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-            const float z = top == -INFINITY ? 0.f : top;
-            const float f0 = exp2f((m0 - z) * DEC_LOG2E), f1 = exp2f((m1 - z) * DEC_LOG2E), f2 = exp2f((m2 - z) * DEC_LOG2E),
-                        f3 = exp2f((m3 - z) * DEC_LOG2E);
-            const float sum = f0 * s_l[0][h] + f1 * s_l[1][h] + f2 * s_l[2][h] + f3 * s_l[3][h];
-            const float out = f0 * s_o[0][h][at] + f1 * s_o[1][h][at] + f2 * s_o[2][h][at] + f3 * s_o[3][h][at];
-            if (direct) {
-                const int m = at / VE, ch = (SMALL ? m * VE : min(m * VE, D - VE)) + at % VE;
-                if (SMALL ? ch < D : m * VE < D)
-                    static_cast<T*>(p.o)[b * p.so[0] + (int64_t)(head0 + h) * p.so[1] + ch] = from_f32<T>(sum == 0.f ? 0.f : out / sum);
-                if (p.lse && at == 0) p.lse[(int64_t)b * p.Hq + head0 + h] = sum == 0.f ? -INFINITY : z + logf(sum);
+                    for (int e = 0; e < VE; ++e) out[e] = from_f32<T>(l == 0.f ? 0.f : acc[e][r] * inv);
+                    if constexpr (SMALL) {
+#pragma unroll
+                        for (int e = 0; e < VE; ++e)
+                            if (first + e < D) orow[first + e] = out[e];
+                    } else {
+                        if (first < D) __builtin_memcpy(orow + min(first, D - VE), out, sizeof(out));
+                    }
+                }
+                if (p.lse && g == 0) p.lse[(int64_t)b * p.Hq + head0 + n16] = l == 0.f ? -INFINITY : (ref == -INFINITY ? 0.f : ref) + logf(l);
             } else {
-                slot[h * DP + at] = out;
-                if (at == 0) {
-                    slot[p.part_rows * DP + h] = top;
-                    slot[p.part_rows * DP + 16 + h] = sum;
+                float* slot = p.part + (int64_t)(2 * blockIdx.x + (begins ? 1 : 0)) * ((int64_t)p.part_rows * DP + 32);
+                float out[4 * VE];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) out[r * VE + e] = acc[e][r];
+                f32x4* to = reinterpret_cast<f32x4*>(slot + n16 * DP + 4 * g * VE);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) to[i] = f32x4{out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]};
+                if (g == 0) {
+                    slot[p.part_rows * DP + n16] = ref;
+                    slot[p.part_rows * DP + 16 + n16] = l;
                 }
             }
         }
@@ -452,12 +451,14 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const DecodeParams p,
     }
 }
 
-// One workgroup per (sequence, query head): joins the pieces of its unit, in order.  32 lanes take 4 channels each, 8 groups of
-// lanes every eighth piece.
-template <typename T, int NC, bool SMALL> __global__ __launch_bounds__(256) void paged_decode_merge_kernel(const DecodeParams p) {
-    constexpr int DP = 32 * NC, VE = DP / 16;
-    __shared__ float s_o[8][DP];
-    __shared__ float s_sum[8], s_top[8];
+// One workgroup of THREADS per (sequence, query head): joins the pieces of its unit, in order.  32 lanes take 4 channels each, G
+// groups of lanes every G-th piece, eight at a time in flight.
+template <typename T, int NC, bool SMALL, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(const DecodeParams p) {
+    constexpr int DP = 32 * NC, VE = DP / 16, G = THREADS / 32, BATCH = 8 * G;
+    __shared__ float s_o[G][DP];
+    __shared__ float s_f[BATCH];
+    __shared__ float s_red[THREADS / 64];
     const int b = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
     const int hk = h / p.group, in_group = h - hk * p.group;
     const int unit = hk * p.head_tiles + (in_group >> 4), row = in_group & 15;
@@ -466,31 +467,46 @@ template <typename T, int NC, bool SMALL> __global__ __launch_bounds__(256) void
     const int64_t slot_size = (int64_t)p.part_rows * DP + 32;
     auto slot = [&](int w) { return p.part + (int64_t)(2 * w + (w == span.x ? 1 : 0)) * slot_size; };
     const int tid = threadIdx.x, grp = tid >> 5, c4 = (tid & 31) * 4;
+    auto over_all = [&](float v, auto op) {  // v over the workgroup, op(a, b)
+        __syncthreads();
+        if ((tid & 63) == 0) s_red[tid >> 6] = v;
+        __syncthreads();
+        v = s_red[0];
+        for (int i = 1; i < THREADS / 64; ++i) v = op(v, s_red[i]);
+        return v;
+    };
     float top = -INFINITY;
-    for (int w = span.x + tid; w <= span.y; w += 256) top = fmaxf(top, slot(w)[p.part_rows * DP + row]);
-    top = group_reduce<64, OpMax>(top);
-    if ((tid & 63) == 0) s_top[tid >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    for (int w = span.x + tid; w <= span.y; w += THREADS) top = fmaxf(top, slot(w)[p.part_rows * DP + row]);
+    top = over_all(group_reduce<64, OpMax>(top), [](float a, float c) { return fmaxf(a, c); });
     const float z = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int w = span.x + grp; w <= span.y; w += 8) {
-        const float* s = slot(w);
-        const float f = exp2f((s[p.part_rows * DP + row] - z) * DEC_LOG2E);
-        sum += f * s[p.part_rows * DP + 16 + row];
-        if (c4 < DP) o += f * *reinterpret_cast<const f32x4*>(s + row * DP + c4);
+    for (int w0 = span.x; w0 <= span.y; w0 += BATCH) {
+        if (tid < BATCH) {
+            float f = 0.f;
+            if (w0 + tid <= span.y) {
+                const float* s = slot(w0 + tid) + p.part_rows * DP + row;
+                f = exp2f((s[0] - z) * DEC_LOG2E);
+                sum += f * s[16];
+            }
+            s_f[tid] = f;
+        }
+        __syncthreads();
+        if (c4 < DP) {
+            f32x4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = w0 + i * G + grp <= span.y ? *reinterpret_cast<const f32x4*>(slot(w0 + i * G + grp) + row * DP + c4) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o += s_f[i * G + grp] * v[i];
+        }
+        __syncthreads();
     }
     if (c4 < DP) *reinterpret_cast<f32x4*>(&s_o[grp][c4]) = o;
-    if ((tid & 31) == 0) s_sum[grp] = sum;
-    __syncthreads();
-    sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum += s_sum[i];
+    sum = over_all(group_reduce<64>(sum), [](float a, float c) { return a + c; });
     if (tid < DP) {
         float out = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out += s_o[i][tid];
+        for (int i = 0; i < G; ++i) out += s_o[i][tid];
         const int m = tid / VE, ch = (SMALL ? m * VE : min(m * VE, p.D - VE)) + tid % VE;
         if (SMALL ? ch < p.D : m * VE < p.D)
             static_cast<T*>(p.o)[b * p.so[0] + (int64_t)h * p.so[1] + ch] = from_f32<T>(sum == 0.f ? 0.f : out / sum);

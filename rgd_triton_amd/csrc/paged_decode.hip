@@ -5,20 +5,28 @@
 
 namespace {
 
-// Workgroups of the decode launch: DEC_WAVES_PER_SIMD resident on every compute unit.
-constexpr int DEC_WAVES_PER_SIMD = 2;
-int64_t decode_grid() { return (int64_t)rgd_num_cus() * DEC_WAVES_PER_SIMD; }
+#ifndef DEC_WPS
+#define DEC_WPS 2
+#endif
+#ifndef DEC_LEAST
+#define DEC_LEAST 1
+#endif
+// Wavefronts of the decode launch
+int64_t decode_grid() { return (int64_t)rgd_num_cus() * 4 * DEC_WPS; }
 
 int chunks_of(int64_t D) { return (int)((D + 31) / 32); }
 
 template <typename T, int NC, bool PAGE8, bool SMALL>
 int decode_launch(const DecodeParams& p, const DecodeBias* rel, unsigned grid, bool merge, hipStream_t s) {
-    const hipError_t e = rel ? rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, true>, dim3(grid), dim3(256), 0, s, p, *rel)
-                             : rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, false>, dim3(grid), dim3(256), 0, s, p, DecodeNoBias{});
+    const hipError_t e = rel ? rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, true>, dim3(grid), dim3(64), 0, s, p, *rel)
+                             : rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, false>, dim3(grid), dim3(64), 0, s, p, DecodeNoBias{});
     const int rc = rgd_launch_status("rgd_paged_decode", e);
     if (rc != RGD_OK || !merge) return rc;
-    return rgd_launch_status("rgd_paged_decode", rgd_launch(paged_decode_merge_kernel<T, NC, SMALL>, dim3((unsigned)p.B * (unsigned)p.Hq),
-                                                            dim3(256), 0, s, p));
+    // pieces of a unit, if all units are alike: beyond what the small workgroup keeps in flight at once the large one is faster
+    const dim3 heads((unsigned)p.B * (unsigned)p.Hq);
+    const bool many = grid / ((int64_t)p.B * p.units) > 64;
+    return rgd_launch_status("rgd_paged_decode", many ? rgd_launch(paged_decode_merge_kernel<T, NC, SMALL, 1024>, heads, dim3(1024), 0, s, p)
+                                                      : rgd_launch(paged_decode_merge_kernel<T, NC, SMALL, 256>, heads, dim3(256), 0, s, p));
 }
 
 template <typename T> int decode_dispatch(const DecodeParams& p, const DecodeBias* rel, unsigned grid, bool merge, hipStream_t s) {
@@ -109,12 +117,13 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
     p.num_pages = (int)num_pages;
     p.div_page = make_fastdiv((uint32_t)page_size);
     p.scale = softmax_scale;
+    p.least = DEC_LEAST;
     hipStream_t s = static_cast<hipStream_t>(stream);
     RGD_REQUIRE(workspace && workspace_bytes >= rgd_paged_decode_workspace(B, Hq, Hkv, D), RGD_ERR_WORKSPACE,
                 "%s: workspace of %zu bytes, needs %zu", name, workspace_bytes, rgd_paged_decode_workspace(B, Hq, Hkv, D));
     p.plan = static_cast<int2*>(workspace);
     p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (B * p.units * (int64_t)sizeof(int2) + 15) / 16 * 16);
-    // more workgroups than there can be tiles have nothing to do; units of one tile are in no two workgroups
+    // more wavefronts than there can be tiles have nothing to do; units of one tile are in no two wavefronts
     const int64_t most = p.capacity > DEC_TILE ? (p.capacity + DEC_TILE - 1) / DEC_TILE : 1;
     const int64_t tiles = B * p.units * most;
     const unsigned grid = (unsigned)(tiles < decode_grid() ? tiles : decode_grid());
