@@ -361,10 +361,13 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
  * no bucket has two ranges; starts and buckets are HOST arrays, read during the call; at most 256 ranges and buckets.
  * ------------------------------------------------------------------------------------------ */
 
-/* bias by (head, row) strides (stride_h, stride_n), any dtype */
+/* bias by (head, row) strides (stride_h, stride_n), any dtype.  Scratch (any contents on entry, 16-byte aligned; 0 bytes for
+ * matrices up to 64 MB): with it a large matrix is written in address order; without it (NULL or smaller), or where the size is
+ * 0, by one launch, with the same results. */
+size_t rgd_rel_bias_fwd_workspace(int64_t H, int64_t Tq, int64_t Tk, int bias_dtype);
 int rgd_rel_bias_fwd(int64_t H, int64_t Tq, int64_t Tk, const void* weight, int64_t w_stride, int64_t num_buckets,
                      int w_dtype, int64_t n_ranges, const int32_t* starts, const int32_t* buckets, int64_t q_offset,
-                     const rgd_tensor4* bias, int bias_dtype, void* stream);
+                     const rgd_tensor4* bias, int bias_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* dweight[b * dw_stride + h] = sum of dbias[h, i, j] over the pairs whose d lies in bucket b (0 for a bucket without a range):
  * fp32 sums in a fixed order, rounded once to the weight's type.  Scratch: any contents on entry, 16-byte aligned. */

@@ -75,7 +75,8 @@ _SIGNATURES = {
     "rgd_paged_decode_workspace": (_sz, [_i64] * 4),
     "rgd_paged_decode": (_int, [_i64] * 4 + [_vp] * 3 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, _i64, _vp, _vp,
                                                          _vp, _vp, _int, _f32, _vp, _sz, _vp]),
-    "rgd_rel_bias_fwd": (_int, [_i64] * 3 + [_vp, _i64, _i64, _int, _i64, _vp, _vp, _i64, _vp, _int, _vp]),
+    "rgd_rel_bias_fwd_workspace": (_sz, [_i64] * 3 + [_int]),
+    "rgd_rel_bias_fwd": (_int, [_i64] * 3 + [_vp, _i64, _i64, _int, _i64, _vp, _vp, _i64, _vp, _int, _vp, _sz, _vp]),
     "rgd_rel_bias_bwd_workspace": (_sz, [_i64] * 4),
     "rgd_rel_bias_bwd": (_int, [_i64] * 3 + [_vp, _int, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _int, _vp, _sz, _vp]),
 }

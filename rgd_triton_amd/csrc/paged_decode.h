@@ -55,6 +55,7 @@ struct DecodeBias {  // relative bias: weight (buckets, Hq), ranges of the dista
     const void* w;
     int64_t w_stride;
     int w_dtype, n_ranges;
+    int half;  // largest power of two below n_ranges (0 for one range)
     int start[DEC_MAX_RANGES], bucket[DEC_MAX_RANGES];
 };
 struct DecodeNoBias {};  // (2 KB less to hand over with every launch)
@@ -109,14 +110,15 @@ constexpr float DEC_LAZY = 5.5f;
 // What is left is at most (2^-7 + 2^-8) p, its own rounding 2^-14.4 p.
 constexpr float DEC_HIGH = 1.0f - 1.0f / 128;
 
-// NC: 32-channel chunks of the head dim (DP = 32 NC).  PAGE8: the page size is a multiple of 8, so the 8 keys of a lane group
-// stand in one page and a lane needs two page numbers; otherwise the lanes look up the 32 keys' pages together and pass
-// the row addresses around.  SMALL: D < 8, rows are read element by element.
-template <typename T, int NC, bool PAGE8, bool SMALL, bool BIAS>
-__global__ __launch_bounds__(64) void paged_decode_kernel(const DecodeParams p,
+// NC: 32-channel chunks of the head dim (DP = 32 NC).  SMALL: D < 8, rows are read element by element.
+// The lanes look up the 32 keys' pages together and pass the row addresses around (20 cross-lane moves a step), whatever the
+// page size: a variant for pages of whole groups of 8 keys, in which a lane needs two page numbers and no moves, was no faster
+// ((19 x 24 heads, D = 128, lengths to 2000) pages of 16: 54.4 us this way, 54.1 that).
+template <typename T, int NC, bool SMALL, bool BIAS>
+__global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams p,
                                                           const std::conditional_t<BIAS, DecodeBias, DecodeNoBias> rel) {
     constexpr int DP = 32 * NC, VE = DP / 16, VW = VE / 2;
-    __shared__ int s_start[BIAS ? DEC_MAX_RANGES : 1];
+    __shared__ int s_start[BIAS ? DEC_MAX_RANGES : 1], s_bucket[BIAS ? DEC_MAX_RANGES : 1];
     __shared__ float s_w[BIAS ? DEC_MAX_RANGES : 1][16];
 
     const int lane = threadIdx.x;
@@ -127,6 +129,14 @@ __global__ __launch_bounds__(64) void paged_decode_kernel(const DecodeParams p,
         return n < 0 ? 0 : (n < p.capacity ? n : p.capacity);
     };
     auto tiles_of = [](int len) { return len > 0 ? (int)(((uint32_t)len + DEC_TILE - 1) / DEC_TILE) : 1; };
+
+    if constexpr (BIAS) {  // (starts filled up to the next power of two: a search halves it)
+        for (int r = lane; r < DEC_MAX_RANGES; r += 64) {
+            s_start[r] = r < rel.n_ranges ? (r == 0 ? INT32_MIN : rel.start[r]) : INT32_MAX;
+            s_bucket[r] = r < rel.n_ranges ? rel.bucket[r] : 0;
+        }
+        __syncthreads();  // (one wavefront: orders its LDS accesses)
+    }
 
     // ---- this wavefront's run of tiles [x, x_end) and the sequence it begins in
     auto scan = [&](uint32_t n) {  // inclusive sum over the lanes (64 sequences of at most 2^26 tiles)
@@ -189,37 +199,25 @@ __global__ __launch_bounds__(64) void paged_decode_kernel(const DecodeParams p,
         uint32_t vr[8][VW];
         // Page numbers are looked up two steps ahead and turned into row addresses one step ahead: loads return in order, so a
         // lookup behind a step's loads would hold up the next step's until those are there.
-        int e0 = 0, e1 = 0;                // PAGE8: page numbers of the lane's keys and values; else e0: of key t + lane % 32
-        int64_t koff = 0, voff = 0;        // row offsets: PAGE8: of the lane's first key and value; else: of key t + lane % 32
-        uint64_t ok_cur = 0, ok_next = 0;  // ballot of "the page exists": PAGE8: of the lane's values; else: bit i for key t + i
+        int entry = 0;                     // page number of key t + lane % 32
+        int64_t koff = 0, voff = 0;        // its row offsets
+        uint32_t ok_cur = 0, ok_next = 0;  // bit i: the page of key t + i exists
 
-        auto lookup = [&](int t) __attribute__((always_inline)) {  // (clamped: only the sequence's own page numbers are read)
-            if constexpr (PAGE8) {
-                e0 = table[fast_div(min(t + 8 * (n16 >> 2), (len - 1) & ~7), p.div_page)];
-                e1 = table[fast_div(min(t + 8 * g, (len - 1) & ~7), p.div_page)];
-            } else {
-                e0 = table[fast_div(min(t + (lane & 31), len - 1), p.div_page)];
-            }
-        };
+        auto token = [&](int t) { return min(t + (lane & 31), len - 1); };  // (only the sequence's own page numbers are read)
+        auto lookup = [&](int t) __attribute__((always_inline)) { entry = table[fast_div(token(t), p.div_page)]; };
         auto locate = [&](int t) __attribute__((always_inline)) {
-            auto slot_of = [&](int tok) { return tok - (int)(fast_div(tok, p.div_page) * p.div_page.d); };
-            const bool ok0 = e0 >= 0 && e0 < p.num_pages;
-            if constexpr (PAGE8) {
-                const bool ok1 = e1 >= 0 && e1 < p.num_pages;
-                ok_next = __ballot(ok1);
-                koff = (ok0 ? e0 : 0) * p.sk[0] + (slot_of(min(t + 8 * (n16 >> 2), (len - 1) & ~7)) + (n16 & 3)) * p.sk[2];
-                voff = (ok1 ? e1 : 0) * p.sv[0] + slot_of(min(t + 8 * g, (len - 1) & ~7)) * p.sv[2];
-            } else {
-                const int slot = slot_of(min(t + (lane & 31), len - 1));
-                ok_next = __ballot(ok0);
-                koff = (ok0 ? e0 : 0) * p.sk[0] + slot * p.sk[2];
-                voff = (ok0 ? e0 : 0) * p.sv[0] + slot * p.sv[2];
-            }
+            const int tok = token(t);
+            const int slot = tok - (int)(fast_div(tok, p.div_page) * p.div_page.d);
+            const bool ok = entry >= 0 && entry < p.num_pages;
+            const int64_t page = ok ? entry : 0;
+            ok_next = (uint32_t)__ballot(ok);
+            koff = page * p.sk[0] + slot * p.sk[2];
+            voff = page * p.sv[0] + slot * p.sv[2];
         };
         auto load_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
-                const T* row = kbase + (PAGE8 ? koff + 4 * a * p.sk[2] : __shfl(koff, 8 * (n16 >> 2) + 4 * a + (n16 & 3), 64));
+                const T* row = kbase + __shfl(koff, 8 * (n16 >> 2) + 4 * a + (n16 & 3), 64);
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     if constexpr (SMALL) {
@@ -238,7 +236,7 @@ __global__ __launch_bounds__(64) void paged_decode_kernel(const DecodeParams p,
         auto load_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const T* row = vbase + (PAGE8 ? voff + i * p.sv[2] : __shfl(voff, 8 * g + i, 64));
+                const T* row = vbase + __shfl(voff, 8 * g + i, 64);
                 if constexpr (SMALL) {
                     const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
                     vr[i][0] = r[min(vstart, D - 1)] | (uint32_t)r[min(vstart + 1, D - 1)] << 16;
@@ -269,6 +267,19 @@ __global__ __launch_bounds__(64) void paged_decode_kernel(const DecodeParams p,
             qf[c] = raw.v;
             kmask = keep.v;
         }
+        if constexpr (BIAS) {  // the weight of the unit's heads, by range
+            const int hb = heads > 1 ? 32 - __builtin_clz(heads - 1) : 0;
+#pragma unroll 4
+            for (int i = lane; i < rel.n_ranges << hb; i += 64) {
+                const int r = i >> hb, h = min(i - (r << hb), heads - 1);
+                const int64_t at = s_bucket[r] * rel.w_stride + head0 + h;
+                s_w[r][h] = rel.w_dtype == RGD_F32 ? static_cast<const float*>(rel.w)[at]
+                            : rel.w_dtype == RGD_F16 ? to_f32(static_cast<const f16_t*>(rel.w)[at])
+                                                     : to_f32(static_cast<const bf16_t*>(rel.w)[at]);
+            }
+            __syncthreads();  // (one wavefront: orders its LDS accesses)
+        }
+
         f32x4 acc[VE];
 #pragma unroll
         for (int e = 0; e < VE; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -288,8 +299,8 @@ __global__ __launch_bounds__(64) void paged_decode_kernel(const DecodeParams p,
                     s[a] = Mfma16<T>::run(kk, qf[c], s[a]);
                 }
             }
-            const bool whole = t + 32 <= len && (PAGE8 ? ok_cur == ~0ull : (uint32_t)ok_cur == ~0u);
-            const uint32_t ok8 = PAGE8 ? ((ok_cur >> lane) & 1 ? 0xFFu : 0u) : (uint32_t)ok_cur >> (8 * g);  // of the lane's 8 keys
+            const bool whole = t + 32 <= len && ok_cur == ~0u;
+            const uint32_t ok8 = ok_cur >> (8 * g);  // of the lane's 8 keys
             if (prefetch) {
                 locate(t + DEC_TILE);
                 lookup(t + 2 * DEC_TILE);
@@ -305,17 +316,15 @@ __global__ __launch_bounds__(64) void paged_decode_kernel(const DecodeParams p,
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x8[i] += wv;
                 } else {
-                    int lo = 0, hi = rel.n_ranges - 1;  // last range that begins at or before d0
-                    while (lo < hi) {
-                        const int mid = (lo + hi + 1) >> 1;
-                        if (s_start[mid] <= d0) lo = mid;
-                        else hi = mid - 1;
+                    int at[8];  // last range that begins at or before the key's distance, the 8 searches side by side
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) at[i] = 0;
+                    for (int half = rel.half; half > 0; half >>= 1) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) at[i] += s_start[at[i] + half] <= d0 + i ? half : 0;
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        while (lo + 1 < rel.n_ranges && s_start[lo + 1] <= d0 + i) ++lo;
-                        x8[i] += s_w[lo][hrow];
-                    }
+                    for (int i = 0; i < 8; ++i) x8[i] += s_w[at[i]][hrow];
                 }
             }
             if (!whole) {
@@ -377,19 +386,6 @@ __global__ __launch_bounds__(64) void paged_decode_kernel(const DecodeParams p,
             __builtin_amdgcn_sched_barrier(0);  // (keys before values here as in the loop: waits count loads in order)
             load_v();
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (BIAS) {  // the weight of the unit's heads, by range
-                const int hb = heads > 1 ? 32 - __builtin_clz(heads - 1) : 0;
-#pragma unroll 4
-                for (int i = lane; i < rel.n_ranges << hb; i += 64) {
-                    const int r = i >> hb, h = min(i - (r << hb), heads - 1);
-                    const int64_t at = rel.bucket[r] * rel.w_stride + head0 + h;
-                    s_w[r][h] = rel.w_dtype == RGD_F32 ? static_cast<const float*>(rel.w)[at]
-                                : rel.w_dtype == RGD_F16 ? to_f32(static_cast<const f16_t*>(rel.w)[at])
-                                                         : to_f32(static_cast<const bf16_t*>(rel.w)[at]);
-                    if (i == r << hb) s_start[r] = r == 0 ? INT32_MIN : rel.start[r];
-                }
-                __syncthreads();  // (one wavefront: orders its LDS accesses)
-            }
             const int t_last = (tile1 - 1) * DEC_TILE;
             for (int t = t0; t < t_last; t += DEC_TILE) {
                 ok_cur = ok_next;

@@ -16,10 +16,10 @@ int64_t decode_grid() { return (int64_t)rgd_num_cus() * 4 * DEC_WPS; }
 
 int chunks_of(int64_t D) { return (int)((D + 31) / 32); }
 
-template <typename T, int NC, bool PAGE8, bool SMALL>
+template <typename T, int NC, bool SMALL>
 int decode_launch(const DecodeParams& p, const DecodeBias* rel, unsigned grid, bool merge, hipStream_t s) {
-    const hipError_t e = rel ? rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, true>, dim3(grid), dim3(64), 0, s, p, *rel)
-                             : rgd_launch(paged_decode_kernel<T, NC, PAGE8, SMALL, false>, dim3(grid), dim3(64), 0, s, p, DecodeNoBias{});
+    const hipError_t e = rel ? rgd_launch(paged_decode_kernel<T, NC, SMALL, true>, dim3(grid), dim3(64), 0, s, p, *rel)
+                             : rgd_launch(paged_decode_kernel<T, NC, SMALL, false>, dim3(grid), dim3(64), 0, s, p, DecodeNoBias{});
     const int rc = rgd_launch_status("rgd_paged_decode", e);
     if (rc != RGD_OK || !merge) return rc;
     // pieces of a unit, if all units are alike: beyond what the small workgroup keeps in flight at once the large one is faster
@@ -30,13 +30,12 @@ int decode_launch(const DecodeParams& p, const DecodeBias* rel, unsigned grid, b
 }
 
 template <typename T> int decode_dispatch(const DecodeParams& p, const DecodeBias* rel, unsigned grid, bool merge, hipStream_t s) {
-    if (p.D < 8) return decode_launch<T, 1, false, true>(p, rel, grid, merge, s);
-    const bool page8 = p.div_page.d % 8 == 0;
+    if (p.D < 8) return decode_launch<T, 1, true>(p, rel, grid, merge, s);
     switch (chunks_of(p.D)) {
-        case 1: return page8 ? decode_launch<T, 1, true, false>(p, rel, grid, merge, s) : decode_launch<T, 1, false, false>(p, rel, grid, merge, s);
-        case 2: return page8 ? decode_launch<T, 2, true, false>(p, rel, grid, merge, s) : decode_launch<T, 2, false, false>(p, rel, grid, merge, s);
-        case 3: return page8 ? decode_launch<T, 3, true, false>(p, rel, grid, merge, s) : decode_launch<T, 3, false, false>(p, rel, grid, merge, s);
-        default: return page8 ? decode_launch<T, 4, true, false>(p, rel, grid, merge, s) : decode_launch<T, 4, false, false>(p, rel, grid, merge, s);
+        case 1: return decode_launch<T, 1, false>(p, rel, grid, merge, s);
+        case 2: return decode_launch<T, 2, false>(p, rel, grid, merge, s);
+        case 3: return decode_launch<T, 3, false>(p, rel, grid, merge, s);
+        default: return decode_launch<T, 4, false>(p, rel, grid, merge, s);
     }
 }
 
@@ -89,6 +88,7 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
         rel.w_stride = w_stride;
         rel.w_dtype = w_dtype;
         rel.n_ranges = (int)n_ranges;
+        for (rel.half = 0; (rel.half ? 2 * rel.half : 1) < n_ranges;) rel.half = rel.half ? 2 * rel.half : 1;
         bias = &rel;
     }
     p.q = q->ptr;

@@ -6,13 +6,20 @@
 // is the sum of each diagonal, added up over the diagonals of a bucket.  Bound by memory: the matrix is written (forward) or
 // read (backward) once.
 //
-// Both directions walk the matrix along its diagonals.  A wavefront takes a strip of 512 columns and goes down `chunk` rows, 8 rows
-// and 8 columns at a time: lane l holds the 8 x 8 block whose columns begin at strip + 8 l + 8 n in step n, so the 15
-// diagonals of a lane's block are the same in every step.
+// The backward, and the forward of a matrix that fits the Infinity Cache, walk the matrix along its diagonals.  A wavefront takes a
+// strip of 512 columns and goes down `chunk` rows, 8 rows and 8 columns at a time: lane l holds the 8 x 8 block whose columns
+// begin at strip + 8 l + 8 n in step n, so the 15 diagonals of a lane's block are the same in every step.
 //   forward   the 15 values are looked up once, the 8 rows of the block packed once; each step is eight 16-byte stores
-//   backward  15 sums stay in registers; each step is eight 16-byte loads and 64 additions
-// Blocks left of the first or right of the last column are skipped, one that the last column cuts goes element by element.
-// Rows need no alignment: the hardware takes 16-byte accesses at any address.
+//   backward  15 sums stay in registers; each step is eight 16-byte streaming loads and 64 additions
+// Blocks left of the first or right of the last column are skipped.
+// A matrix beyond 64 MB is written in address order instead: the memory takes 6.9 TB/s from workgroups that write 4 KB side by
+// side in the order they are launched, and 4 from the walk, whose workgroups write 8 rows each all over the matrix.  The
+// values of a head's diagonals are first laid out in a row of the workspace (read back from the L2), then each thread takes
+// 8 columns of two rows (one row: too few bytes in flight for a round trip to the L2, 4.4 TB/s; four rows 5.7, two 6.2).
+// bf16, walk / address order: (24, 4352, 4352) 222 / 172 us, (16, 2048, 2048) 33 / 26 us, (16, 1024, 1024) 10.5 / 11 us.
+// Rows need no alignment: those written in address order are cut at the 16-byte boundaries of each row, the walk loads and stores
+// at any address, which the hardware takes.  A block that the last column cuts is read further left and shifted (element
+// by element its wavefront was the last to end: (24, 4352, 4351) bf16 381 us instead of 165).
 #include "common.h"
 
 #include <string.h>
@@ -21,21 +28,27 @@ namespace {
 
 constexpr int MAX_RANGES = 256;
 constexpr int STRIP = 512;
+constexpr int64_t ORDERED_BYTES = int64_t(64) << 20;  // larger matrices are written in address order
+constexpr int VALUES_BEFORE = 8;                      // values in front of the first row's, for a row that begins off a boundary
 
-struct RelRanges {  // range k: start[k] <= d < start[k + 1], ascending, bucket[k]; start[0] covers everything below
+struct RelRanges {  // range k: start[k] <= d < start[k + 1], ascending; start[0] covers everything below; the rest INT32_MAX
     int n;
+    int half;  // largest power of two below n (0 for one range)
     int start[MAX_RANGES];
-    int bucket[MAX_RANGES];
+    int16_t bucket[MAX_RANGES];  // of a range
+    int16_t range[MAX_RANGES];   // of a bucket, -1: none
 };
 
 struct RelParams {
-    const void* w;      // forward: weight; backward: unused
-    void* bias;         // forward: written; backward: dbias, read
-    float* part;        // backward: [head][range][task]
+    const void* w;  // forward: weight
+    void* bias;     // forward: written; backward: dbias, read
+    void* part;     // backward: sums [head][range][task]; forward in address order: values of the diagonals [head][width]
     void* dw;
     int64_t w_stride, stride_h, stride_n;
     int w_dtype, H, Tq, Tk, offset;
-    int chunk, strips, tasks, num_buckets;
+    int chunk, strips, tasks;
+    int width;       // address order: values of a head; value e is that of d = e - VALUES_BEFORE - Tq - offset
+    FastDiv blocks;  // address order: 8-column blocks of a row
     RelRanges r;
 };
 
@@ -43,9 +56,10 @@ struct Split {
     int64_t chunk, chunks, strips, tasks;
 };
 
-// Rows of a task.  Long tasks spend less on their beginning and end (looking values up, adding buckets up) and waste fewer lanes at
+// Rows of a task.  Long tasks spend less on their beginning and end (looking values up, adding ranges up) and waste fewer lanes at
 // the slanted edges, short ones fill the chip: the longest of 16 .. 256 rows that still gives every compute unit 8
-// wavefronts.  (24, 4352, 4352) bf16 forward + backward at 256 / 64 rows: MEASURED_LARGE; (8, 128, 128) at 16 / 256: MEASURED_SMALL.
+// wavefronts.  Backward with 4 / 8 / 16 / 32 of them, bf16: (24, 4352, 4352) 148 / 148 / 153 / 154 us, (16, 2048, 2048)
+// 29 / 28 / 26 / 28 us, (16, 2560, 2560) 37 / 38 / 40 / 42 us.
 Split split(int64_t H, int64_t Tq, int64_t Tk) {
     Split s;
     for (s.chunk = 256;; s.chunk /= 2) {
@@ -56,37 +70,73 @@ Split split(int64_t H, int64_t Tq, int64_t Tk) {
     }
 }
 
-template <typename T> struct Block {  // 8 consecutive elements
-    static constexpr int NW = 8 * sizeof(T) / 4;
-    uint32_t w[NW];
+// 8 consecutive elements at any address: 16-byte accesses, unaligned where the row is
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+template <typename T> struct Block {
+    static constexpr int NV = 8 * sizeof(T) / 16;
+    u32x4 v[NV];
+    // streaming (a gradient is read once): without it (24, 4352, 4352) bf16 takes 237 us instead of 147
+    __device__ __forceinline__ void load(const char* p) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p) + i);
+    }
+    // element e becomes element e + s, zeros from the end (bit operations: choices by a condition would become branches)
+    __device__ __forceinline__ Block down(int s) const {
+        constexpr int N = 4 * NV;
+        uint32_t w[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) w[k] = v[k / 4][k % 4];
+        const int bytes = s * (int)sizeof(T);
+#pragma unroll
+        for (int d = N / 2; d >= 1; d /= 2) {  // by d dwords
+            const uint32_t m = 0u - (bytes / (4 * d) & 1);
+#pragma unroll
+            for (int k = 0; k < N; ++k) w[k] = ((k + d < N ? w[k + d] : 0u) & m) | (w[k] & ~m);
+        }
+        Block b;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            b.v[k / 4][k % 4] = sizeof(T) == 2 ? __builtin_amdgcn_alignbyte(k + 1 < N ? w[k + 1] : 0u, w[k], bytes & 2) : w[k];
+        return b;
+    }
+    __device__ __forceinline__ void fetch(const T* p) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = reinterpret_cast<const u32x4_any*>(p)[i];
+    }
+    __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) reinterpret_cast<u32x4_any*>(p)[i] = v[i];
+    }
 };
 
-// W column of the workgroup's head and the starts of the ranges in LDS
-__device__ __forceinline__ void stage_ranges(const RelParams& p, int* s_start) {
-    for (int k = threadIdx.x; k < p.r.n; k += 256) s_start[k] = k == 0 ? INT32_MIN : p.r.start[k];
+__device__ __forceinline__ float load_dyn(const void* p, int dtype, int64_t i) {
+    return dtype == RGD_F32 ? static_cast<const float*>(p)[i]
+           : dtype == RGD_F16 ? to_f32(static_cast<const f16_t*>(p)[i]) : to_f32(static_cast<const bf16_t*>(p)[i]);
 }
 
-__device__ __forceinline__ int find_range(const int* s_start, int n, int d) {  // last range that begins at or before d
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s_start[mid] <= d) lo = mid;
-        else hi = mid - 1;
+// the range starts and the weight of head h by range, for the workgroup
+__device__ __forceinline__ void stage_weight(const RelParams& p, int h, int* s_start, float* s_w) {
+    const int k = threadIdx.x;  // 256 threads, 256 ranges at most
+    s_start[k] = k == 0 ? INT32_MIN : p.r.start[k];
+    if (k < p.r.n) s_w[k] = load_dyn(p.w, p.w_dtype, p.r.bucket[k] * p.w_stride + h);
+    __syncthreads();
+}
+
+// for N distances d, d + 1, ..: the last range that begins at or before each (starts beyond n are INT32_MAX), side by side
+template <int N> __device__ __forceinline__ void find_ranges(const int* s_start, int half, int d, int (&at)[N]) {
+#pragma unroll
+    for (int a = 0; a < N; ++a) at[a] = 0;
+    for (; half > 0; half >>= 1) {
+#pragma unroll
+        for (int a = 0; a < N; ++a) at[a] += s_start[at[a] + half] <= d + a ? half : 0;
     }
-    return lo;
 }
 
 template <typename T> __global__ __launch_bounds__(256) void rel_bias_fwd_kernel(const RelParams p) {
     __shared__ int s_start[MAX_RANGES];
     __shared__ float s_w[MAX_RANGES];
     const int h = blockIdx.y;
-    stage_ranges(p, s_start);
-    for (int k = threadIdx.x; k < p.r.n; k += 256) {
-        const int64_t at = p.r.bucket[k] * p.w_stride + h;
-        s_w[k] = p.w_dtype == RGD_F32 ? static_cast<const float*>(p.w)[at]
-                 : p.w_dtype == RGD_F16 ? to_f32(static_cast<const f16_t*>(p.w)[at]) : to_f32(static_cast<const bf16_t*>(p.w)[at]);
-    }
-    __syncthreads();
+    stage_weight(p, h, s_start, s_w);
     const int task = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     if (task >= p.tasks) return;
     const int c = task / p.strips, strip = (task - c * p.strips) * STRIP - (p.chunk - 8);
@@ -95,13 +145,10 @@ template <typename T> __global__ __launch_bounds__(256) void rel_bias_fwd_kernel
 
     T v[15];
     {
-        const int d0 = col - i0 - 7 - p.offset;
-        int k = find_range(s_start, p.r.n, d0);
+        int at[15];
+        find_ranges(s_start, p.r.half, col - i0 - 7 - p.offset, at);
 #pragma unroll
-        for (int a = 0; a < 15; ++a) {
-            while (k + 1 < p.r.n && s_start[k + 1] <= d0 + a) ++k;
-            v[a] = from_f32<T>(s_w[k]);
-        }
+        for (int a = 0; a < 15; ++a) v[a] = from_f32<T>(s_w[at[a]]);
     }
     Block<T> row[8];
 #pragma unroll
@@ -113,7 +160,7 @@ template <typename T> __global__ __launch_bounds__(256) void rel_bias_fwd_kernel
         if (col < 0 || col >= p.Tk) continue;
         if (n + 8 <= rows && col + 8 <= p.Tk) {
 #pragma unroll
-            for (int r = 0; r < 8; ++r) __builtin_memcpy(out + r * step, &row[r], sizeof(row[r]));
+            for (int r = 0; r < 8; ++r) row[r].store(reinterpret_cast<T*>(out + r * step));
         } else {
 #pragma unroll
             for (int r = 0; r < 8; ++r)
@@ -126,13 +173,53 @@ template <typename T> __global__ __launch_bounds__(256) void rel_bias_fwd_kernel
     }
 }
 
+// the values of a head's diagonals, in the bias type
+template <typename T> __global__ __launch_bounds__(256) void rel_bias_values_kernel(const RelParams p) {
+    __shared__ int s_start[MAX_RANGES];
+    __shared__ float s_w[MAX_RANGES];
+    const int h = blockIdx.y, e = blockIdx.x * 256 + threadIdx.x;
+    stage_weight(p, h, s_start, s_w);
+    if (e >= p.width) return;
+    int at[1];
+    find_ranges(s_start, p.r.half, e - VALUES_BEFORE - p.Tq - p.offset, at);
+    static_cast<T*>(p.part)[(int64_t)h * p.width + e] = from_f32<T>(s_w[at[0]]);
+}
+
+// thread: 8 columns of rows 2 rb and 2 rb + 1, in each row from the 16-byte boundary at or before column 8 cb
+template <typename T> __global__ __launch_bounds__(256) void rel_bias_ordered_kernel(const RelParams p) {
+    const uint32_t c = blockIdx.x * 256 + threadIdx.x;
+    const uint32_t rb = fast_div(c, p.blocks), cb = c - rb * p.blocks.d;
+    const int h = blockIdx.y;
+    const T* values = static_cast<const T*>(p.part) + (int64_t)h * p.width;
+    Block<T> v[2];
+    T* row[2];
+    int col[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int i = min(2 * (int)rb + r, p.Tq - 1);
+        row[r] = static_cast<T*>(p.bias) + h * p.stride_h + i * p.stride_n;
+        col[r] = 8 * (int)cb - (int)(reinterpret_cast<uintptr_t>(row[r]) % 16 / sizeof(T));
+        v[r].fetch(values + (col[r] - i + p.Tq + VALUES_BEFORE));
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        if (2 * (int)rb + r >= p.Tq) break;
+        if (col[r] >= 0 && col[r] + 8 <= p.Tk) {
+            v[r].store(row[r] + col[r]);
+        } else {
+            T one[8];
+            __builtin_memcpy(one, &v[r], sizeof(one));
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col[r] + e >= 0 && col[r] + e < p.Tk) row[r][col[r] + e] = one[e];
+        }
+    }
+}
+
 // part[(h * ranges + k) * tasks + task]: what the task adds to range k
 template <typename T> __global__ __launch_bounds__(256) void rel_bias_bwd_kernel(const RelParams p) {
-    __shared__ int s_start[MAX_RANGES];
-    __shared__ float s_sum[4][STRIP + 8];
+    __shared__ double s_sum[4][STRIP + 8];
     const int h = blockIdx.y;
-    stage_ranges(p, s_start);
-    __syncthreads();
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int task = blockIdx.x * 4 + wave;
     if (task >= p.tasks) return;
@@ -143,19 +230,39 @@ template <typename T> __global__ __launch_bounds__(256) void rel_bias_bwd_kernel
     float acc[15];
 #pragma unroll
     for (int a = 0; a < 15; ++a) acc[a] = 0.f;
-    const char* in = static_cast<const char*>(p.bias) + (h * p.stride_h + i0 * p.stride_n) * (int64_t)sizeof(T) + col * (int64_t)sizeof(T);
     const int64_t step = p.stride_n * (int64_t)sizeof(T);
-    for (int n = 0; n < rows; n += 8, col += 8, in += 8 * step + 8 * (int64_t)sizeof(T)) {
-        if (col < 0 || col >= p.Tk) continue;
-        if (n + 8 <= rows && col + 8 <= p.Tk) {
-            T x[8][8];
+    const char* in = static_cast<const char*>(p.bias) + (h * p.stride_h + i0 * p.stride_n) * (int64_t)sizeof(T) + col * (int64_t)sizeof(T);
+    const int over = (8 - p.Tk % 8) % 8;  // columns that a block cut by the last column lacks: it is read that much further left
+    if (p.Tk >= 8) {
+        for (int n = 0; n < rows; n += 8, col += 8, in += 8 * step + 8 * (int64_t)sizeof(T)) {
+            if (col < 0 || col >= p.Tk) continue;
+            const bool cut = col + 8 > p.Tk;
+            const char* from = in - (cut ? over * (int)sizeof(T) : 0);
+            const int left = rows - n;
+            Block<T> x[8];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) __builtin_memcpy(x[r], in + r * step, sizeof(x[r]));
+            for (int r = 0; r < 8; ++r) x[r].load(from + min(r, left - 1) * step);
+            if (__any(cut)) {
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
+                for (int r = 0; r < 8; ++r) {
+                    const Block<T> y = x[r].down(over);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) acc[e - r + 7] += to_f32(x[r][e]);
-        } else {
+                    for (int i = 0; i < Block<T>::NV; ++i) x[r].v[i] = cut ? y.v[i] : x[r].v[i];
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                if (r < left) {
+                    T row[8];
+                    __builtin_memcpy(row, &x[r], sizeof(row));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[e - r + 7] += to_f32(row[e]);
+                }
+            }
+        }
+    } else {  // rows shorter than a block: element by element
+        for (int n = 0; n < rows; n += 8, col += 8, in += 8 * step + 8 * (int64_t)sizeof(T)) {
+            if (col < 0 || col >= p.Tk) continue;
 #pragma unroll
             for (int r = 0; r < 8; ++r)
 #pragma unroll
@@ -164,45 +271,62 @@ template <typename T> __global__ __launch_bounds__(256) void rel_bias_bwd_kernel
         }
     }
 
-    // diagonal 8 l + a of the strip: the lane's sum and, for a < 7, its left neighbour's a + 8
-    float* sum = s_sum[wave];
+    // Diagonal 8 l + a of the strip is the lane's sum and, for a < 7, its left neighbour's a + 8; the last lane's a + 8 are the
+    // last seven.
+    float line[8];
 #pragma unroll
     for (int a = 0; a < 8; ++a) {
-        float v = acc[a];
+        line[a] = acc[a];
         if (a < 7) {
             const float left = __shfl_up(acc[a + 8], 1, 64);
-            v += lane > 0 ? left : 0.f;
+            line[a] += lane > 0 ? left : 0.f;
         }
-        sum[8 * lane + a] = v;
     }
-    if (lane == 63) {
+    // Ranges are differences of the diagonals' running sum, which is kept in 64 bits: a short range behind a long one loses
+    // nothing.
+    double* sum = s_sum[wave];
+    double total = line[0];
 #pragma unroll
-        for (int a = 8; a < 15; ++a) sum[STRIP + a - 8] = acc[a];
+    for (int a = 1; a < 8; ++a) total += line[a];
+    const double own = total;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const double up = __shfl_up(total, m, 64);
+        if (lane >= m) total += up;
+    }
+    const bool finite = __all(isfinite(total));
+    double run = finite ? total - own : 0.;  // (an infinity or NaN stays in its own range: those sums are made one by one)
+    if (lane == 0) sum[0] = 0.;
+#pragma unroll
+    for (int a = 0; a < 15; ++a) {
+        if (a >= 8 && lane < 63) break;
+        const float v = a < 8 ? line[a & 7] : acc[a];
+        run = finite ? run + v : v;
+        sum[8 * lane + a + 1] = run;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (a wavefront's own LDS rows: its accesses are in order)
     __builtin_amdgcn_wave_barrier();
     const int d0 = strip - i0 - 7 - p.offset;  // d of the first of STRIP + 7 diagonals
-    float* out = p.part + (int64_t)h * p.r.n * p.tasks + task;
-    for (int k = 0; k < p.r.n; ++k) {
-        const int lo = k == 0 ? 0 : max(0, s_start[k] - d0);
-        const int hi = k + 1 < p.r.n ? min(STRIP + 7, s_start[k + 1] - d0) : STRIP + 7;
-        float s = 0.f;
-        if (lo < hi) {
-            for (int e = lo + lane; e < hi; e += 64) s += sum[e];
-            s = group_reduce<64>(s);
+    float* out = static_cast<float*>(p.part) + (int64_t)h * p.r.n * p.tasks + task;
+    for (int k = lane; k < p.r.n; k += 64) {
+        const int lo = k == 0 ? 0 : (int)min((int64_t)STRIP + 7, max((int64_t)0, (int64_t)p.r.start[k] - d0));
+        const int hi = k + 1 < p.r.n ? (int)min((int64_t)STRIP + 7, max((int64_t)0, (int64_t)p.r.start[k + 1] - d0)) : STRIP + 7;
+        double s = sum[hi] - sum[lo];
+        if (!finite) {
+            s = 0.;
+            for (int e = lo; e < hi; ++e) s += sum[e + 1];
         }
-        if (lane == 0) out[(int64_t)k * p.tasks] = s;
+        out[(int64_t)k * p.tasks] = (float)s;
     }
 }
 
 // one wavefront per (head, bucket): the tasks' sums in a fixed order
 __global__ __launch_bounds__(64) void rel_bias_bucket_kernel(const RelParams p) {
     const int b = blockIdx.x, h = blockIdx.y;
-    int k = -1;
-    for (int i = 0; i < p.r.n; ++i) k = p.r.bucket[i] == b ? i : k;
+    const int k = p.r.range[b];
     float s = 0.f;
     if (k >= 0) {
-        const float* row = p.part + ((int64_t)h * p.r.n + k) * p.tasks;
+        const float* row = static_cast<const float*>(p.part) + ((int64_t)h * p.r.n + k) * p.tasks;
         float s4[4] = {0.f, 0.f, 0.f, 0.f};
         int t = threadIdx.x;
         for (; t + 192 < p.tasks; t += 256) {
@@ -252,17 +376,48 @@ void fill(RelParams* p, int64_t H, int64_t Tq, int64_t Tk, int64_t n_ranges, con
         p->stride_n = bias->stride_n;
     }
     p->r.n = (int)n_ranges;
-    memcpy(p->r.start, starts, n_ranges * sizeof(int));
-    memcpy(p->r.bucket, buckets, n_ranges * sizeof(int));
+    for (p->r.half = 0; (p->r.half ? 2 * p->r.half : 1) < n_ranges;) p->r.half = p->r.half ? 2 * p->r.half : 1;
+    for (int k = 0; k < MAX_RANGES; ++k) {
+        p->r.start[k] = k < n_ranges ? starts[k] : INT32_MAX;
+        p->r.range[k] = -1;
+    }
+    for (int k = 0; k < n_ranges; ++k) {
+        p->r.bucket[k] = (int16_t)buckets[k];
+        p->r.range[buckets[k]] = (int16_t)k;
+    }
+}
+
+// values of a head's diagonals: VALUES_BEFORE, then d = -Tq - offset .. Tk - 1 - offset, then what the last block holds beyond: it
+// begins at column Tk + 6 at most, value VALUES_BEFORE + Tq + Tk + 6 in the first row
+int64_t values_of(int64_t Tq, int64_t Tk) { return (VALUES_BEFORE + Tq + Tk + 6 + 8 + 7) / 8 * 8; }
+
+template <typename T> int ordered(const char* name, RelParams& p, hipStream_t s) {
+    const int64_t es = sizeof(T);
+    const bool aligned = rgd_aligned16(p.bias) && p.stride_n * es % 16 == 0 && p.stride_h * es % 16 == 0;
+    p.blocks = make_fastdiv((uint32_t)((p.Tk + (aligned ? 7 : 14)) / 8));  // (one more where rows begin off a boundary)
+    const dim3 values((unsigned)((p.width + 255) / 256), (unsigned)p.H);
+    const int rc = rgd_launch_status(name, rgd_launch(rel_bias_values_kernel<T>, values, dim3(256), 0, s, p));
+    if (rc != RGD_OK) return rc;
+    const int64_t blocks = (int64_t)((p.Tq + 1) / 2) * p.blocks.d;
+    const dim3 grid((unsigned)((blocks + 255) / 256), (unsigned)p.H);
+    return rgd_launch_status(name, rgd_launch(rel_bias_ordered_kernel<T>, grid, dim3(256), 0, s, p));
 }
 
 }  // namespace
 
 extern "C" {
 
+size_t rgd_rel_bias_fwd_workspace(int64_t H, int64_t Tq, int64_t Tk, int bias_dtype) {
+    const int64_t lim = int64_t(1) << 30;
+    if (H <= 0 || Tq <= 0 || Tk <= 0 || Tq >= lim || Tk >= lim || !rgd_dtype_ok(bias_dtype)) return 0;
+    const int64_t es = rgd_dtype_size(bias_dtype);
+    if (H * ((double)Tq * Tk * es) <= (double)ORDERED_BYTES || ((Tq + 1) / 2) * ((Tk + 14) / 8) >= (int64_t(1) << 31) - 256) return 0;
+    return (size_t)(H * values_of(Tq, Tk) * es);
+}
+
 int rgd_rel_bias_fwd(int64_t H, int64_t Tq, int64_t Tk, const void* weight, int64_t w_stride, int64_t num_buckets, int w_dtype,
                      int64_t n_ranges, const int32_t* starts, const int32_t* buckets, int64_t q_offset, const rgd_tensor4* bias,
-                     int bias_dtype, void* stream) {
+                     int bias_dtype, void* workspace, size_t workspace_bytes, void* stream) {
     const char* name = "rgd_rel_bias_fwd";
     rgd_ensure_init();
     RGD_REQUIRE(rgd_dtype_ok(w_dtype) && rgd_dtype_ok(bias_dtype), RGD_ERR_INVALID, "%s: Only support fp16, bf16, and fp32", name);
@@ -274,8 +429,14 @@ int rgd_rel_bias_fwd(int64_t H, int64_t Tq, int64_t Tk, const void* weight, int6
     p.w = weight;
     p.w_stride = w_stride;
     p.w_dtype = w_dtype;
-    const dim3 grid((unsigned)((p.tasks + 3) / 4), (unsigned)H);
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (workspace && workspace_bytes > 0 && workspace_bytes >= rgd_rel_bias_fwd_workspace(H, Tq, Tk, bias_dtype) &&
+        rgd_rel_bias_fwd_workspace(H, Tq, Tk, bias_dtype) > 0) {
+        p.part = workspace;
+        p.width = (int)values_of(Tq, Tk);
+        return bias_dtype == RGD_F16 ? ordered<f16_t>(name, p, s) : bias_dtype == RGD_BF16 ? ordered<bf16_t>(name, p, s) : ordered<float>(name, p, s);
+    }
+    const dim3 grid((unsigned)((p.tasks + 3) / 4), (unsigned)H);
     const hipError_t e = bias_dtype == RGD_F16 ? rgd_launch(rel_bias_fwd_kernel<f16_t>, grid, dim3(256), 0, s, p)
                          : bias_dtype == RGD_BF16 ? rgd_launch(rel_bias_fwd_kernel<bf16_t>, grid, dim3(256), 0, s, p)
                                                   : rgd_launch(rel_bias_fwd_kernel<float>, grid, dim3(256), 0, s, p);

@@ -780,10 +780,13 @@ def _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, kernel_c
             return _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, None)
     num_buckets, nheads = weight.shape
     bias = torch.empty((1, nheads, seqlen_q, seqlen_k), dtype=dtype, device=device)
-    rc = _hip.lib().rgd_rel_bias_fwd(nheads, seqlen_q, seqlen_k, weight.data_ptr(), wstride[0], num_buckets,
-                                     _hip.dtype_code(weight.dtype), ranges.n, ranges.c_starts, ranges.c_buckets, q_offset,
-                                     _desc4(bias.data_ptr(), 0, seqlen_q * seqlen_k, seqlen_k), _hip.dtype_code(dtype),
-                                     _raw_stream(index))
+    lib, code = _hip.lib(), _hip.dtype_code(dtype)
+    nbytes = lib.rgd_rel_bias_fwd_workspace(nheads, seqlen_q, seqlen_k, code)  # 0 for all but large matrices
+    ws = _hip.workspace(device, nbytes) if nbytes else None
+    rc = lib.rgd_rel_bias_fwd(nheads, seqlen_q, seqlen_k, weight.data_ptr(), wstride[0], num_buckets, _hip.dtype_code(weight.dtype),
+                              ranges.n, ranges.c_starts, ranges.c_buckets, q_offset,
+                              _desc4(bias.data_ptr(), 0, seqlen_q * seqlen_k, seqlen_k), code, ws.data_ptr() if nbytes else None, nbytes,
+                              _raw_stream(index))
     if rc:
         _hip.check(rc, "rgd_rel_bias_fwd")
     return bias

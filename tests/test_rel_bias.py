@@ -200,3 +200,48 @@ def test_rel_bias_forward_in_a_graph_and_backward_refused():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("H,Tq,Tk,off,dtype", [(5, 2601, 2603, 0, torch.bfloat16), (4, 3001, 2808, -700, torch.float16), (3, 2560, 2400, 0, torch.float32),
+                                               (2, 2049, 4101, 2052, torch.float32), (1, 3, 11200001, 0, torch.bfloat16), (16, 2200001, 1, 9, torch.bfloat16),
+                                               (9, 1040, 4096, 3056, torch.bfloat16)])
+def test_rel_bias_large(H, Tq, Tk, off, dtype):
+    """matrices beyond 64 MB, which are written in address order: every value, the same bits without scratch (the walk of small
+    matrices), nothing written outside of rows with gaps, and the gradient"""
+    from rgd_triton_amd import _hip, relative_position_bias_fn
+    from rgd_triton_amd.functional import relative_ranges
+
+    nb, md = 32, 128
+    g = gen(40)
+    w = randn(g, nb, H).cuda().requires_grad_(True)
+    bias = relative_position_bias_fn(w, Tq, Tk, max_distance=md, bidirectional=True, q_offset=off, dtype=dtype)
+    # row i of a head is the window of its diagonals' values that begins at Tq - 1 - i
+    d = torch.arange(-(Tq - 1), Tk, device="cuda") - off
+    near = torch.tensor([serving_oracle.bucket_of(x, nb, md, True) for x in range(-md, md + 1)], device="cuda")
+    bucket = near[d.clamp(-md, md) + md]
+    values = w.detach().t()[:, bucket].to(dtype)
+    assert torch.equal(bias.detach()[0], values.unfold(1, Tk, 1).flip(1))
+    lib, r = _hip.lib(), relative_ranges(nb, md, True)
+    assert lib.rgd_rel_bias_fwd_workspace(H, Tq, Tk, _hip.dtype_code(dtype)) > 0
+    walk = torch.empty_like(bias)
+    rc = lib.rgd_rel_bias_fwd(H, Tq, Tk, w.data_ptr(), H, nb, 0, r.n, r.c_starts, r.c_buckets, off, _hip.desc4(walk.data_ptr(), 0, Tq * Tk, Tk),
+                              _hip.dtype_code(dtype), None, 0, _hip.stream_ptr(w.device))
+    assert rc == 0 and torch.equal(walk, bias)
+    if Tk < 10**6:
+        gaps = torch.full((H, Tq + 1, Tk + 5), 7.0, dtype=dtype, device="cuda")
+        n = lib.rgd_rel_bias_fwd_workspace(H, Tq, Tk, _hip.dtype_code(dtype))
+        ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        rc = lib.rgd_rel_bias_fwd(H, Tq, Tk, w.data_ptr(), H, nb, 0, r.n, r.c_starts, r.c_buckets, off,
+                                  _hip.desc4(gaps.data_ptr() + 2 * gaps.element_size(), 0, gaps.stride(0), gaps.stride(1)), _hip.dtype_code(dtype),
+                                  ws.data_ptr(), n, _hip.stream_ptr(w.device))
+        assert rc == 0 and torch.equal(gaps[:, :Tq, 2:Tk + 2], bias[0])
+        assert (gaps[:, Tq] == 7).all() and (gaps[:, :, :2] == 7).all() and (gaps[:, :, Tk + 2:] == 7).all()
+    # whole numbers whose sums stay below 2^24: the gradient is exact whatever the order
+    dy = torch.randint(0, 2, (1, 1, Tq, Tk), device="cuda", dtype=torch.int8).to(dtype)
+    (dw,) = torch.autograd.grad(bias, w, dy.expand(1, H, Tq, Tk))
+    ref = torch.zeros(nb, dtype=torch.int64, device="cuda")
+    for i0 in range(0, Tq, max(1, 10**7 // Tk)):
+        i1 = min(Tq, i0 + max(1, 10**7 // Tk))
+        rel = torch.arange(Tk, device="cuda")[None] - torch.arange(i0, i1, device="cuda")[:, None] - off
+        ref.index_add_(0, near[rel.clamp(-md, md) + md].flatten(), dy[0, 0, i0:i1].flatten().long())
+    assert torch.equal(dw.long(), ref[:, None].expand(nb, H)), (dw[:, 0].long() - ref)

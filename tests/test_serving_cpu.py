@@ -145,7 +145,7 @@ def test_rel_bias_refusals():
     ids, twice = (ctypes.c_int32 * 3)(2, 1, 0), (ctypes.c_int32 * 3)(0, 1, 1)
 
     def fwd(**kw):
-        a = dict(H=2, Tq=4, Tk=4, w=BUF, ws=2, nb=3, wdt=0, n=3, starts=up, buckets=ids, off=0, bias=T4, bdt=0)
+        a = dict(H=2, Tq=4, Tk=4, w=BUF, ws=2, nb=3, wdt=0, n=3, starts=up, buckets=ids, off=0, bias=T4, bdt=0, work=None, bytes=0)
         a.update(kw)
         return lib.rgd_rel_bias_fwd(*a.values(), None)
 
@@ -166,6 +166,9 @@ def test_rel_bias_refusals():
     assert bwd(bytes=16) == -4 and b"workspace" in err()
     assert lib.rgd_rel_bias_bwd_workspace(0, 5, 5, 8) == 0 and lib.rgd_rel_bias_bwd_workspace(3, 5, 5, 8) > 0
     assert fwd(Tq=0) == 0
+    # scratch only where the matrix is written in address order: beyond 64 MB
+    assert lib.rgd_rel_bias_fwd_workspace(8, 2048, 2048, 2) == 0 and lib.rgd_rel_bias_fwd_workspace(8, 2048, 2049, 2) > 0
+    assert lib.rgd_rel_bias_fwd_workspace(8, 2048, 2048, 0) > 0 and lib.rgd_rel_bias_fwd_workspace(1, 1 << 30, 8, 0) == 0
 
 
 def test_ranges_refusals():
