@@ -4,21 +4,28 @@
 //   pos = cache_lens[b] + t,  slot = (page_table[b][pos / page_size], pos % page_size)
 //   y_c = x_c cos[pos][c] + rot(x)_c sin[pos][c] for c < R and pos < cutoff, x_c elsewhere;  rot(x)_(2i, 2i+1) = (-x_(2i+1), x_2i)
 //
-// Bound by memory: every new row is read once and written once.  A row of D <= 128 elements belongs to G consecutive lanes,
-// VEC elements each (16 bytes where pointers and strides allow), so a rotary pair stays inside a lane and the row's mean and
-// variance are sums over G lanes.  Statistics and rotation are fp32, rounded once to the tensor type.
+// Bound by memory: every new row is read once and written once.  A row of D <= 128 elements belongs to G consecutive lanes, 8
+// elements each, so a rotary pair stays inside a lane and the row's mean and variance are sums over G lanes.  The last lane's
+// 8 begin at D - 8 where D is no multiple of 8 (where D is even it writes some elements a second time, the same); accesses are 16 bytes at any
+// address, which the hardware takes.  Statistics and rotation are fp32, rounded once to the tensor type.
+// A lane group takes U = 2 heads of one token: their rows are in flight together, and the token's length, page number, sine
+// and cosine, each a round trip behind the other, are read once for both.  U = 1 / 2 / 4 / 8: 8 prompts of 4096 tokens (32 and
+// 8 heads, D = 128, bf16, fp32 table) 166 / 144 / 143 / 151 us (839 MB: 5.8 TB/s, a large copy reaches 5.4), one token each
+// of 256 sequences 5.1 / 5.2 / 5.8 / 7.4 us.  Streaming loads gain 2 % there and cost 13 % on rows that are still cached.
 #include "common.h"
 
 #include <string.h>
 
 namespace {
 
+constexpr int APPEND_HEADS = 2;  // heads of a token that a lane group takes (U above)
+
 struct AppendRows {  // one of q, k, v
     const void* x;
     void* y;             // q: output (batch, head, token); k, v: cache (page, head, slot)
     int64_t sx[3], sy[3];  // (batch, head, token) and (batch or page, head, token or slot)
-    uint32_t rows, heads, n_inner;
-    FastDiv div_b, div_inner;  // by heads * T and by the inner extent
+    uint32_t groups, heads;    // (sequence, token, U heads)
+    FastDiv div_b, div_inner;  // by the groups of a sequence and by the inner extent
     int token_inner;
     int cutoff;
 };
@@ -37,106 +44,159 @@ struct AppendParams {
     FastDiv div_page;
     const void* pe;
     int64_t pe_ss, pe_sn;
-    int pe_dtype;
 };
 
-template <typename T, int G, int VEC, bool VECTOR, bool LN>
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+// N elements of a row from `at` on as floats.  WIDE: 16-byte loads at any address; else element by element, those beyond `limit`
+// repeat the last.
+template <typename T, int N, bool WIDE> __device__ __forceinline__ void load_row(const T* row, int at, int limit, T (&out)[N]) {
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < N * (int)sizeof(T) / 16; ++i) {
+            const u32x4 v = reinterpret_cast<const u32x4_any*>(row + at)[i];
+            __builtin_memcpy(reinterpret_cast<char*>(out) + 16 * i, &v, 16);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) out[e] = row[min(at + e, limit - 1)];
+    }
+}
+
+template <typename TP, int N, bool WIDE> __device__ __forceinline__ void load_table(const void* row, int at, int R, float (&out)[N]) {
+    TP v[N];
+    if (WIDE && at + N <= R) load_row<TP, N, true>(static_cast<const TP*>(row), at, R, v);
+    else load_row<TP, N, false>(static_cast<const TP*>(row), at, R, v);  // (the rotary dim ends inside the lane's elements)
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = to_f32(v[e]);
+}
+
+// TP: element type of the rotary table.  WIDE: D >= 8 and 8 elements a lane; else 2, element by element.
+template <typename T, typename TP, int G, bool WIDE, bool LN>
 __global__ __launch_bounds__(256) void cache_append_kernel(const AppendParams p) {
-    constexpr int ROWS = 256 / G;
+    constexpr int GROUPS = 256 / G, VEC = WIDE ? 8 : 2, U = APPEND_HEADS;
     const int which = blockIdx.x < p.blocks_q ? 0 : (blockIdx.x < p.blocks_q + p.blocks_k ? 1 : 2);
     const AppendRows& a = p.t[which];
     const uint32_t block0 = which == 0 ? 0u : (which == 1 ? p.blocks_q : p.blocks_q + p.blocks_k);
-    const uint32_t row = (blockIdx.x - block0) * ROWS + threadIdx.x / G;
-    if (row >= a.rows) return;  // whole lane groups leave: the reductions below stay inside a group
-    const int first = (threadIdx.x % G) * VEC;
+    const uint32_t group = (blockIdx.x - block0) * GROUPS + threadIdx.x / G;
+    if (group >= a.groups) return;  // whole lane groups leave: the reductions below stay inside a group
     const int D = p.D;
+    const int own = (threadIdx.x % G) * VEC;             // the lane's elements of the row: those from `own` on are no other lane's
+    const int first = WIDE ? min(own, D - VEC) : own;    // (WIDE: a lane behind the row's end repeats the last 8)
 
-    const uint32_t b = fast_div(row, a.div_b);
-    const uint32_t in_b = row - b * a.div_b.d;
+    const uint32_t b = fast_div(group, a.div_b);
+    const uint32_t in_b = group - b * a.div_b.d;
     const uint32_t outer = fast_div(in_b, a.div_inner);
     const uint32_t inner = in_b - outer * a.div_inner.d;
-    const uint32_t head = a.token_inner ? outer : inner;
+    const uint32_t head0 = (a.token_inner ? outer : inner) * U;
     const uint32_t tok = a.token_inner ? inner : outer;
 
-    Chunk<T, VEC, VECTOR> c;
-    c.load(static_cast<const T*>(a.x) + b * a.sx[0] + head * a.sx[1] + tok * a.sx[2], first, D);
+    const T* from = static_cast<const T*>(a.x) + b * a.sx[0] + tok * a.sx[2];
+    T raw[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_row<T, VEC, WIDE>(from + min(head0 + u, a.heads - 1) * a.sx[1], first, D, raw[u]);
     const int64_t pos = static_cast<int64_t>(p.cache_lens[b]) + tok;
     const bool live = pos >= 0 && pos < p.capacity && (!p.new_lens || static_cast<int>(tok) < p.new_lens[b]);
     T* y = static_cast<T*>(a.y);
+    const bool turn = which != 2 && live && first < p.R && pos < a.cutoff;
+    float sin[VEC], cos[VEC];
+    if (turn) {
+        const TP* row = static_cast<const TP*>(p.pe) + pos * p.pe_sn;
+        load_table<TP, VEC, WIDE>(row, first, p.R, sin);
+        load_table<TP, VEC, WIDE>(row + p.pe_ss, first, p.R, cos);
+    }
     if (which == 0) {
-        y += b * a.sy[0] + head * a.sy[1] + tok * a.sy[2];
+        y += b * a.sy[0] + tok * a.sy[2];
     } else {
         if (!live) return;
         const uint32_t entry = fast_div(static_cast<uint32_t>(pos), p.div_page);
         const int page = p.page_table[b * p.table_stride + entry];
         if (page < 0 || page >= p.num_pages) return;  // no such page: the token is not stored
         const uint32_t slot = static_cast<uint32_t>(pos) - entry * p.div_page.d;
-        y += page * a.sy[0] + head * a.sy[1] + slot * a.sy[2];
+        y += page * a.sy[0] + slot * a.sy[2];
     }
-    float x[VEC];
-    c.decode(first, D, x);
-    if (!live) {  // a padded query row
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x[e] = 0.f;
-        store_chunk<T, VEC, VECTOR>(y, first, D, x);
-        return;
-    }
-    if (which != 2) {
-        if constexpr (LN) {
+    for (int u = 0; u < U; ++u) {
+        float x[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = to_f32(raw[u][e]);
+        if (LN && which != 2) {
             float s = 0.f;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s += x[e];
+            for (int e = 0; e < VEC; ++e) s += first + e >= own && first + e < D ? x[e] : 0.f;
             const float mean = group_reduce<G>(s) * p.inv_d;
             s = 0.f;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 x[e] -= mean;
-                s += first + e < D ? x[e] * x[e] : 0.f;
+                s += first + e >= own && first + e < D ? x[e] * x[e] : 0.f;
             }
             const float rstd = rsqrtf(group_reduce<G>(s) * p.inv_d + p.eps);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) x[e] *= rstd;
         }
-        if (first < p.R && pos < a.cutoff) {
-            const int ps = p.pe_dtype == RGD_F32 ? 4 : 2;
-            const char* sn = static_cast<const char*>(p.pe) + pos * p.pe_sn * ps;
-            float sin[VEC], cos[VEC], out[VEC];
-            load_chunk_dyn<VEC, VECTOR>(sn, p.pe_dtype, first, p.R, sin);
-            load_chunk_dyn<VEC, VECTOR>(sn + p.pe_ss * ps, p.pe_dtype, first, p.R, cos);
+        if (turn) {
+            float out[VEC];
+            if (WIDE && (D & 1)) {  // the last lane's elements begin at an odd channel: pairs by the channel's parity
 #pragma unroll
-            for (int e = 0; e < VEC; e += 2) {
-                out[e] = x[e] * cos[e] - x[e + 1] * sin[e];
-                out[e + 1] = x[e + 1] * cos[e + 1] + x[e] * sin[e + 1];
+                for (int e = 0; e < VEC; ++e) {
+                    const float even = x[e] * cos[e] - (e + 1 < VEC ? x[e + 1] : 0.f) * sin[e];
+                    const float odd = x[e] * cos[e] + (e > 0 ? x[e - 1] : 0.f) * sin[e];
+                    out[e] = (first + e) & 1 ? odd : even;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) {
+                    out[e] = x[e] * cos[e] - x[e + 1] * sin[e];
+                    out[e + 1] = x[e + 1] * cos[e + 1] + x[e] * sin[e + 1];
+                }
             }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) x[e] = first + e < p.R ? out[e] : x[e];
         }
+        if (head0 + u < a.heads && own < D) {
+            T* to = y + (head0 + u) * a.sy[1] + first;
+            T out[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) out[e] = from_f32<T>(live ? x[e] : 0.f);  // (a padded query row is zero)
+            if (WIDE && !(first & 1)) {
+                u32x4 v;
+                __builtin_memcpy(&v, out, VEC * sizeof(T));
+                *reinterpret_cast<u32x4_any*>(to) = v;
+            } else {  // (from an odd channel on the first element's partner is missing: only the lane's own are written)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (first + e >= own && first + e < D) to[e] = out[e];
+            }
+        }
     }
-    store_chunk<T, VEC, VECTOR>(y, first, D, x);
 }
 
-bool vec_ok(const rgd_tensor4* t) {
-    return rgd_aligned16(t->ptr) && t->stride_b % 8 == 0 && t->stride_h % 8 == 0 && t->stride_n % 8 == 0;
-}
-
-template <typename T, int G, int VEC, bool VECTOR>
-int append_launch(AppendParams& p, bool ln, hipStream_t s) {
-    const uint32_t rows = 256 / G;
+template <typename T, typename TP, int G, bool WIDE>
+int append_launch(AppendParams& p, int64_t B, int64_t tokens, bool ln, hipStream_t s) {
     uint32_t blocks[3];
-    for (int i = 0; i < 3; ++i) blocks[i] = (p.t[i].rows + rows - 1) / rows;
+    for (int i = 0; i < 3; ++i) {
+        AppendRows& a = p.t[i];
+        const uint32_t chunks = (a.heads + APPEND_HEADS - 1) / APPEND_HEADS;
+        a.groups = (uint32_t)(B * tokens * chunks);
+        a.div_b = make_fastdiv((uint32_t)(tokens * chunks));
+        a.div_inner = make_fastdiv(a.token_inner ? (uint32_t)tokens : chunks);
+        blocks[i] = (a.groups + 256 / G - 1) / (256 / G);
+    }
     p.blocks_q = blocks[0];
     p.blocks_k = blocks[1];
     const dim3 grid(blocks[0] + blocks[1] + blocks[2]);
-    const hipError_t e = ln ? rgd_launch(cache_append_kernel<T, G, VEC, VECTOR, true>, grid, dim3(256), 0, s, p)
-                            : rgd_launch(cache_append_kernel<T, G, VEC, VECTOR, false>, grid, dim3(256), 0, s, p);
+    if (grid.x == 0) return RGD_OK;
+    const hipError_t e = ln ? rgd_launch(cache_append_kernel<T, TP, G, WIDE, true>, grid, dim3(256), 0, s, p)
+                            : rgd_launch(cache_append_kernel<T, TP, G, WIDE, false>, grid, dim3(256), 0, s, p);
     return rgd_launch_status("rgd_rope_cache_append", e);
 }
 
-template <typename T> int append_dispatch(AppendParams& p, bool vector, bool ln, hipStream_t s) {
-    if (!vector) return append_launch<T, 64, 2, false>(p, ln, s);
-    if (p.D <= 32) return append_launch<T, 4, 8, true>(p, ln, s);
-    if (p.D <= 64) return append_launch<T, 8, 8, true>(p, ln, s);
-    return append_launch<T, 16, 8, true>(p, ln, s);
+template <typename T, typename TP> int append_dispatch(AppendParams& p, int64_t B, int64_t tokens, bool ln, hipStream_t s) {
+    if (p.D < 8) return append_launch<T, TP, 4, false>(p, B, tokens, ln, s);
+    if (p.D <= 32) return append_launch<T, TP, 4, true>(p, B, tokens, ln, s);
+    if (p.D <= 64) return append_launch<T, TP, 8, true>(p, B, tokens, ln, s);
+    return append_launch<T, TP, 16, true>(p, B, tokens, ln, s);
 }
 
 }  // namespace
@@ -171,14 +231,12 @@ extern "C" int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t H
                 "%s: pos_emb must cover every position of the page table", name);
 
     AppendParams p;
-    memset(&p, 0, sizeof(p));
+    memset(&p, 0, sizeof(p));  // (heads 0: nothing to do for a tensor)
     const rgd_tensor4* xs[3] = {q, k, v};
     const rgd_tensor4* ys[3] = {qo, k_cache, v_cache};
-    bool vector = D % 8 == 0;
     for (int i = 0; i < 3; ++i) {
         AppendRows& a = p.t[i];
         const int64_t heads = i == 0 ? Hq : Hkv;
-        a.div_b = a.div_inner = make_fastdiv(1);
         if (heads == 0 || (i && num_pages == 0)) continue;
         RGD_REQUIRE(xs[i] && xs[i]->ptr && ys[i] && ys[i]->ptr, RGD_ERR_INVALID, "%s: null tensor", name);
         a.x = xs[i]->ptr;
@@ -187,17 +245,9 @@ extern "C" int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t H
         a.sy[0] = ys[i]->stride_b, a.sy[1] = ys[i]->stride_h, a.sy[2] = ys[i]->stride_n;
         // rows in memory order of the input: the index with the smaller stride is the inner one
         a.token_inner = xs[i]->stride_n <= xs[i]->stride_h;
-        a.rows = (uint32_t)(B * heads * T);
         a.heads = (uint32_t)heads;
-        a.div_b = make_fastdiv((uint32_t)(heads * T));
-        a.div_inner = make_fastdiv((uint32_t)(a.token_inner ? T : heads));
         const int64_t cutoff = i == 0 ? q_cutoff : k_cutoff;
         a.cutoff = (int)(cutoff < 0 ? 0 : (cutoff < lim - 1 ? cutoff : lim - 1));
-        vector = vector && vec_ok(xs[i]) && vec_ok(ys[i]);
-    }
-    if (R > 0) {  // the table is read with the same width as the tensors
-        const int64_t ps = rgd_dtype_size(pe_dtype);
-        vector = vector && rgd_aligned16(pos_emb) && (pe_stride_s * ps) % 16 == 0 && (pe_stride_n * ps) % 16 == 0 && R % 8 == 0;
     }
     p.D = (int)D;
     p.T = (int)T;
@@ -214,8 +264,8 @@ extern "C" int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t H
     p.pe = pos_emb;
     p.pe_ss = pe_stride_s;
     p.pe_sn = pe_stride_n;
-    p.pe_dtype = pe_dtype;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return dtype == RGD_F16 ? append_dispatch<f16_t>(p, vector, layer_norm != 0, s)
-                            : append_dispatch<bf16_t>(p, vector, layer_norm != 0, s);
+    const bool ln = layer_norm != 0, wide = pe_dtype == RGD_F32;
+    if (dtype == RGD_F16) return wide ? append_dispatch<f16_t, float>(p, B, T, ln, s) : append_dispatch<f16_t, f16_t>(p, B, T, ln, s);
+    return wide ? append_dispatch<bf16_t, float>(p, B, T, ln, s) : append_dispatch<bf16_t, bf16_t>(p, B, T, ln, s);
 }

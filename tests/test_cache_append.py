@@ -23,6 +23,12 @@ CASES = [  # B, T, Hq, Hkv, D, R, page, dtype, table, layer norm, ragged, heads_
     (2, 6, 2, 1, 1, 0, 3, BF, FP, False, False, False),
     (3, 11, 6, 2, 96, 0, 16, HF, FP, True, False, False),
     (3, 11, 6, 2, 112, 20, 8, BF, BF, False, False, False),
+    (2, 5, 5, 3, 100, 50, 8, BF, BF, True, False, True),
+    (2, 5, 3, 3, 127, 126, 8, HF, FP, True, False, False),
+    (2, 5, 3, 1, 9, 8, 8, BF, FP, False, False, False),
+    (2, 5, 3, 1, 33, 2, 8, HF, HF, True, False, False),
+    (1, 5, 1, 1, 7, 6, 8, BF, FP, True, False, True),
+    (2, 5, 7, 2, 122, 122, 8, HF, FP, False, True, True),
 ]
 
 
@@ -119,8 +125,20 @@ def test_append_bad_pages_and_positions():
 
 
 def test_append_in_place_query_and_version():
-    from rgd_triton_amd import RoPECacheAppend
+    """the C ABI allows the rotated query in the query's own place, also where lanes of a row overlap"""
+    from rgd_triton_amd import RoPECacheAppend, _hip, rope_cache_append_fn
 
+    for D, R in ((64, 64), (100, 60), (59, 58)):
+        case = (2, 3, 3, 4, D, R, 16, BF, FP, True, False, True)
+        s = {n: (None if t is None else t.cuda()) for n, t in _inputs(case, 260).items()}
+        want = rope_cache_append_fn(s["q"], s["k"], s["v"], s["table"], s["k_cache"], s["v_cache"], s["pages"], s["lens"], norm_eps=1e-6)
+        d4 = lambda t, h, n: _hip.desc4(t.data_ptr(), t.stride(0), t.stride(h), t.stride(n))  # noqa: E731
+        rc = _hip.lib().rgd_rope_cache_append(
+            2, 3, 3, 4, D, d4(s["q"], 1, 2), d4(s["k"], 1, 2), d4(s["v"], 1, 2), d4(s["q"], 1, 2), d4(s["k_cache"], 2, 1), d4(s["v_cache"], 2, 1),
+            s["k_cache"].shape[0], 16, s["pages"].data_ptr(), s["pages"].shape[1], s["pages"].stride(0), s["lens"].data_ptr(), None,
+            s["table"].data_ptr(), s["table"].shape[1], R, s["table"].stride(0), s["table"].stride(1), 0, 2**31 - 1, 2**31 - 1, 1, 1e-6, 2,
+            _hip.stream_ptr(s["q"].device))
+        assert rc == 0 and torch.equal(s["q"], want)
     case = (2, 3, 4, 4, 64, 64, 16, BF, FP, False, False, True)
     s = {n: (None if t is None else t.cuda()) for n, t in _inputs(case, 260).items()}
     before = s["k_cache"]._version
