@@ -11,8 +11,11 @@
 // wavefronts share leave partial results in the workspace (at most two per wavefront: one unit begun earlier, one not ended),
 // which the merge launch joins in order.
 //
-// A step.  A wavefront (a workgroup of its own) takes 32 keys at a time, without LDS or barriers, operands straight from memory to registers (v_mfma_f32_16x16x32: A lane l holds row l % 16, k = 8 (l / 16) .. + 7; C lane l holds column l % 16,
-// rows 4 (l / 16) + 0..3):
+// A piece's first loads leave while the piece before ends, so that a wavefront with many short pieces does not wait for each.
+//
+// A step.  A wavefront (a workgroup of its own) takes 32 keys at a time, without LDS or barriers, operands straight from memory
+// to registers (v_mfma_f32_16x16x32: A lane l holds row l % 16, k = 8 (l / 16) .. + 7; C lane l holds column l % 16, rows
+// 4 (l / 16) + 0..3):
 //   S^T = K Q^T, two products of 16 keys.  MFMA row i of product a is key 8 (i / 4) + 4 a + i % 4, so that lane group g = l / 16 ends
 //   up with the logits of keys 8 g .. 8 g + 7 of query head l % 16: the layout P^T has to have as the second product's B operand.
 //   O^T += V^T P^T, one product per element e of a lane's piece of a value row: lane l loads VE = DP / 16 channels from VE (l % 16)
@@ -21,6 +24,12 @@
 // the time.  P is split into two 16-bit parts (a second product each): rounded to one, its error would be as large as the
 // output's own rounding, and the products are free (DEC_HIGH).
 // The running maximum is a reference that moves only when a logit exceeds it by LAZY; sums, maxima and outputs are fp32.
+//
+// Measured (this launch / the merge; a read that streams 512 MB reaches 6.6 TB/s): one sequence of 131000 keys, 32 / 8 heads,
+// D = 128: 86 / 7 us, 6.2 TB/s; 64 sequences to 4100 keys, the same heads: 106 / 5 us, 5.5 TB/s; 19 to 2000 keys, 24 heads,
+// D = 80, bias, pages of 5: 53 / 5 us; one of 200 keys, 16 heads, D = 64: 5.8 / 3.5 us.  What a launch takes beyond its
+// bytes, about 15 us, is the chain of loads in front of the first step (lengths, page numbers, keys), the last steps, in which
+// the wavefronts run out one by one, and the merge.
 #pragma once
 
 #include "attn_common.h"
@@ -45,10 +54,9 @@ struct DecodeParams {
     int D, num_pages;
     FastDiv div_page;
     float scale;
-    int2* plan;        // per unit of the batch: wavefronts its first and last piece are in
+    int* plan;         // per unit of the batch: wavefronts its first and last piece are in
     float* part;       // two slots per wavefront: O [rows][DP], then m [16], l [16]
     int part_rows;     // query heads of a slot
-    int least;         // tiles of a run at least
 };
 
 struct DecodeBias {  // relative bias: weight (buckets, Hq), ranges of the distance and their buckets
@@ -76,11 +84,8 @@ template <> struct Mfma16<f16_t> {
 template <int N> __device__ __forceinline__ void load_dwords(const char* p, uint32_t (&out)[N]) {
     __builtin_memcpy(out, p, 4 * N);
 }
-#ifndef DEC_NT
-#define DEC_NT 1
-#endif
+// streaming: a key or value is read once
 template <int N> __device__ __forceinline__ void stream_dwords(const char* p, uint32_t (&out)[N]) {
-    if constexpr (!DEC_NT) { load_dwords<N>(p, out); return; }
     if constexpr (N == 1) {
         typedef uint32_t V __attribute__((aligned(2)));
         out[0] = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
@@ -100,6 +105,11 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 }
 
 __device__ __forceinline__ float xor_lanes(float v, int m) { return __shfl_xor(v, m, 64); }
+
+// Nothing is scheduled across it.  Waits count loads in order, so the order page numbers, keys, values has to be the same in
+// and in front of the loop; and a step's keys, and its values, leave together: with the arithmetic free to move between them
+// one sequence of 131000 keys took 100 us instead of 95.
+#define DEC_KEEP_LOADS() __builtin_amdgcn_sched_barrier(0)
 
 // log2(e) and how far a logit may exceed the reference before that moves: probabilities stay below e^5.5 = 245
 constexpr float DEC_LOG2E = 1.4426950408889634f;
@@ -153,10 +163,9 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
     int64_t total = last_of(incl);
     for (int b0 = 64; b0 < p.B; b0 += 64) total += last_of(scan(b0 + lane < p.B ? tiles_of(length(b0 + lane)) : 0));
     total *= p.units;
-    const int64_t even = total <= INT32_MAX ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x) : (total + gridDim.x - 1) / gridDim.x;
-    const int64_t share = max(even, (int64_t)p.least);
-    int64_t x = share * blockIdx.x;
-    const int64_t x_end = min(total, x + share);
+    const int64_t even = total <= INT32_MAX ? (int64_t)((uint32_t)total / gridDim.x) : total / gridDim.x, rest = total - even * gridDim.x;
+    int64_t x = even * blockIdx.x + min((int64_t)blockIdx.x, rest);
+    const int64_t x_end = x + even + (blockIdx.x < rest ? 1 : 0);
     if (x >= x_end) return;
     int b = 0;
     int64_t base = 0;  // first tile of sequence b
@@ -174,100 +183,186 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
         incl = scan(mine);
     }
 
-    while (x < x_end) {
-        const int len = __builtin_amdgcn_readfirstlane(length(b));
-        const int ntiles = tiles_of(len);
+    // ---- a piece: tiles tile0 .. tile1 - 1 of one unit
+    struct Piece {
+        int b, unit, len, ntiles, tile0, tile1, head0, heads;
+    };
+    auto piece_at = [&]() {
+        Piece c;
+        c.b = b;
+        c.len = __builtin_amdgcn_readfirstlane(length(b));
+        c.ntiles = tiles_of(c.len);
         const int64_t in_seq = x - base;
-        const int unit = in_seq <= INT32_MAX ? (int)((uint32_t)in_seq / (uint32_t)ntiles) : (int)(in_seq / ntiles);
-        const int tile0 = (int)(in_seq - (int64_t)unit * ntiles);
-        const int tile1 = (int)min((int64_t)ntiles, tile0 + (x_end - x));
-        const int hk = unit / p.head_tiles, head0 = hk * p.group + (unit - hk * p.head_tiles) * 16;
-        const int heads = min(16, (hk + 1) * p.group - head0);
+        c.unit = in_seq <= INT32_MAX ? (int)((uint32_t)in_seq / (uint32_t)c.ntiles) : (int)(in_seq / c.ntiles);
+        c.tile0 = (int)(in_seq - (int64_t)c.unit * c.ntiles);
+        c.tile1 = (int)min((int64_t)c.ntiles, c.tile0 + (x_end - x));
+        const int hk = c.unit / p.head_tiles;
+        c.head0 = hk * p.group + (c.unit - hk * p.head_tiles) * 16;
+        c.heads = min(16, (hk + 1) * p.group - c.head0);
+        return c;
+    };
 
-        const T* kbase = static_cast<const T*>(p.k) + hk * p.sk[1];
-        const T* vbase = static_cast<const T*>(p.v) + hk * p.sv[1];
-        const int32_t* table = p.page_table + b * p.table_stride;
+    u32x4 qf[NC];
+    u32x4 kmask;  // channels of the last chunk that are not an earlier chunk's (all ones where the row is long enough)
+    int kstart[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) kstart[c] = SMALL ? 0 : min((4 * c + g) * 8, D - 8);
+    const int vstart = SMALL ? n16 * VE : min(n16 * VE, D - VE);
 
-        u32x4 qf[NC];
-        u32x4 kmask;  // channels of the last chunk that are not an earlier chunk's (all ones where the row is long enough)
-        int kstart[NC];
-#pragma unroll
-        for (int c = 0; c < NC; ++c) kstart[c] = SMALL ? 0 : min((4 * c + g) * 8, D - 8);
-        const int vstart = SMALL ? n16 * VE : min(n16 * VE, D - VE);
+    // Loads.  Page numbers are looked up two steps ahead and turned into row addresses one step ahead: loads return in order, so
+    // a lookup behind a step's loads would hold up the next step's until those are there.  A piece's first loads are
+    // on their way while the piece before ends: what follows is aimed at the piece that is loaded, not the one worked on.
+    int load_len = 0;
+    const T* kbase = nullptr;
+    const T* vbase = nullptr;
+    const int32_t* table = nullptr;
+    u32x4 kf[2][NC];
+    uint32_t vr[8][VW];
+    int entry = 0;                     // page number of key t + lane % 32
+    int64_t koff = 0, voff = 0;        // its row offsets
+    uint32_t ok_cur = 0, ok_next = 0;  // bit i: the page of key t + i exists
 
-        u32x4 kf[2][NC];
-        uint32_t vr[8][VW];
-        // Page numbers are looked up two steps ahead and turned into row addresses one step ahead: loads return in order, so a
-        // lookup behind a step's loads would hold up the next step's until those are there.
-        int entry = 0;                     // page number of key t + lane % 32
-        int64_t koff = 0, voff = 0;        // its row offsets
-        uint32_t ok_cur = 0, ok_next = 0;  // bit i: the page of key t + i exists
-
-        auto token = [&](int t) { return min(t + (lane & 31), len - 1); };  // (only the sequence's own page numbers are read)
-        auto lookup = [&](int t) __attribute__((always_inline)) { entry = table[fast_div(token(t), p.div_page)]; };
-        auto locate = [&](int t) __attribute__((always_inline)) {
-            const int tok = token(t);
-            const int slot = tok - (int)(fast_div(tok, p.div_page) * p.div_page.d);
-            const bool ok = entry >= 0 && entry < p.num_pages;
-            const int64_t page = ok ? entry : 0;
-            ok_next = (uint32_t)__ballot(ok);
-            koff = page * p.sk[0] + slot * p.sk[2];
-            voff = page * p.sv[0] + slot * p.sv[2];
-        };
-        auto load_k = [&]() __attribute__((always_inline)) {
+    auto aim = [&](const Piece& c) __attribute__((always_inline)) {
+        load_len = c.len;
+        const int hk = c.unit / p.head_tiles;
+        kbase = static_cast<const T*>(p.k) + hk * p.sk[1];
+        vbase = static_cast<const T*>(p.v) + hk * p.sv[1];
+        table = p.page_table + c.b * p.table_stride;
+    };
+    // (only the sequence's own page numbers are read; one without keys reads its first, and what that leads to is not used)
+    auto token = [&](int t) { return min(t + (lane & 31), max(load_len - 1, 0)); };
+    auto lookup = [&](int t) __attribute__((always_inline)) { entry = table[fast_div(token(t), p.div_page)]; };
+    auto locate = [&](int t) __attribute__((always_inline)) {
+        const int tok = token(t);
+        const int slot = tok - (int)(fast_div(tok, p.div_page) * p.div_page.d);
+        const bool ok = entry >= 0 && entry < p.num_pages;
+        const int64_t page = ok ? entry : 0;
+        ok_next = (uint32_t)__ballot(ok);
+        koff = page * p.sk[0] + slot * p.sk[2];
+        voff = page * p.sv[0] + slot * p.sv[2];
+    };
+    auto load_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const T* row = kbase + __shfl(koff, 8 * (n16 >> 2) + 4 * a + (n16 & 3), 64);
+        for (int a = 0; a < 2; ++a) {
+            const T* row = kbase + __shfl(koff, 8 * (n16 >> 2) + 4 * a + (n16 & 3), 64);
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    if constexpr (SMALL) {
-                        Pack16 r;
-#pragma unroll
-                        for (int d = 0; d < 8; ++d) r.h[d] = reinterpret_cast<const uint16_t*>(row)[min(d, D - 1)];
-                        kf[a][c] = r.v;
-                    } else {
-                        uint32_t r[4];
-                        stream_dwords<4>(reinterpret_cast<const char*>(row + kstart[c]), r);
-                        kf[a][c] = u32x4{r[0], r[1], r[2], r[3]};
-                    }
-                }
-            }
-        };
-        auto load_v = [&]() __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const T* row = vbase + __shfl(voff, 8 * g + i, 64);
+            for (int c = 0; c < NC; ++c) {
                 if constexpr (SMALL) {
-                    const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
-                    vr[i][0] = r[min(vstart, D - 1)] | (uint32_t)r[min(vstart + 1, D - 1)] << 16;
+                    Pack16 r;
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) r.h[d] = reinterpret_cast<const uint16_t*>(row)[min(d, D - 1)];
+                    kf[a][c] = r.v;
                 } else {
-                    stream_dwords<VW>(reinterpret_cast<const char*>(row + vstart), vr[i]);
+                    uint32_t r[4];
+                    stream_dwords<4>(reinterpret_cast<const char*>(row + kstart[c]), r);
+                    kf[a][c] = u32x4{r[0], r[1], r[2], r[3]};
                 }
             }
-        };
-
-        // ---- the first step's loads on their way, then what does not depend on them
-        const int t0 = tile0 * DEC_TILE;
-        if (len > 0) lookup(t0);
-        // query: B operand of S^T = K Q^T, head n16, channels of chunk 4 c + g
+        }
+    };
+    auto load_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int ci = (4 * c + g) * 8;
+        for (int i = 0; i < 8; ++i) {
+            const T* row = vbase + __shfl(voff, 8 * g + i, 64);
+            if constexpr (SMALL) {
+                const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
+                vr[i][0] = r[min(vstart, D - 1)] | (uint32_t)r[min(vstart + 1, D - 1)] << 16;
+            } else {
+                stream_dwords<VW>(reinterpret_cast<const char*>(row + vstart), vr[i]);
+            }
+        }
+    };
+
+    // query: B operand of S^T = K Q^T, head n16, channels of chunk 4 c + g
+    auto load_q = [&](const Piece& c) __attribute__((always_inline)) {
+        const T* qrow = static_cast<const T*>(p.q) + c.b * p.sq[0] + (int64_t)(c.head0 + min(n16, c.heads - 1)) * p.sq[1];
+        const uint32_t head_ok = n16 < c.heads ? ~0u : 0u;  // (as bits: a choice would become a branch around each load)
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            const int ci = (4 * k + g) * 8;
             Pack16 raw, keep;
-            const T* qrow = static_cast<const T*>(p.q) + b * p.sq[0] + (int64_t)(head0 + min(n16, heads - 1)) * p.sq[1];
             if constexpr (SMALL) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) raw.h[e] = reinterpret_cast<const uint16_t*>(qrow)[min(e, D - 1)];
             } else {
-                load_dwords<4>(reinterpret_cast<const char*>(qrow + kstart[c]), raw.w);
+                load_dwords<4>(reinterpret_cast<const char*>(qrow + kstart[k]), raw.w);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) keep.h[e] = (SMALL ? ci + e < D : kstart[c] + e >= ci) ? 0xFFFF : 0;
-            raw.v = n16 < heads ? raw.v & keep.v : u32x4{0, 0, 0, 0};
-            qf[c] = raw.v;
+            for (int e = 0; e < 8; ++e) keep.h[e] = (SMALL ? ci + e < D : kstart[k] + e >= ci) ? 0xFFFF : 0;
+            qf[k] = raw.v & keep.v & u32x4{head_ok, head_ok, head_ok, head_ok};
             kmask = keep.v;
         }
+    };
+    // The piece that is worked on is `cur`; `next` is the one behind it, whose first page numbers are being looked up.
+    Piece cur = piece_at(), next = cur;
+    bool worked = false;
+    aim(next);
+    lookup(next.tile0 * DEC_TILE);
+    f32x4 acc[VE];
+    float ref = -INFINITY, l = 0.f;
+    auto finish = [&]() __attribute__((always_inline)) {
+        // the piece's result: lane holds channels VE m + e of head n16 for m = 4 g + r
+        const int heads = cur.heads, head0 = cur.head0;
+        const bool begins = cur.tile0 == 0, ends = cur.tile1 == cur.ntiles;
+        l += xor_lanes(l, 16);
+        l += xor_lanes(l, 32);
+        if (lane == 0) {
+            int* plan = &p.plan[2 * ((int64_t)cur.b * p.units + cur.unit)];
+            if (begins) plan[0] = (int)blockIdx.x;
+            if (ends) plan[1] = (int)blockIdx.x;
+        }
+        if (n16 < heads) {
+            if (begins && ends) {
+                const float inv = l == 0.f ? 0.f : 1.0f / l;
+                T* orow = static_cast<T*>(p.o) + cur.b * p.so[0] + (int64_t)(head0 + n16) * p.so[1];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int first = (4 * g + r) * VE;
+                    T out[VE];
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) out[e] = from_f32<T>(l == 0.f ? 0.f : acc[e][r] * inv);
+                    if constexpr (SMALL) {
+#pragma unroll
+                        for (int e = 0; e < VE; ++e)
+                            if (first + e < D) orow[first + e] = out[e];
+                    } else {
+                        if (first < D) __builtin_memcpy(orow + min(first, D - VE), out, sizeof(out));
+                    }
+                }
+                if (p.lse && g == 0) p.lse[(int64_t)cur.b * p.Hq + head0 + n16] = l == 0.f ? -INFINITY : (ref == -INFINITY ? 0.f : ref) + logf(l);
+            } else {
+                float* slot = p.part + (int64_t)(2 * blockIdx.x + (begins ? 1 : 0)) * ((int64_t)p.part_rows * DP + 32);
+                float out[4 * VE];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) out[r * VE + e] = acc[e][r];
+                f32x4* to = reinterpret_cast<f32x4*>(slot + n16 * DP + 4 * g * VE);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) to[i] = f32x4{out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]};
+                if (g == 0) {
+                    slot[p.part_rows * DP + n16] = ref;
+                    slot[p.part_rows * DP + 16 + n16] = l;
+                }
+            }
+        }
+    };
+    for (;;) {
+        // (one place for these loads: at a second one the registers would differ, and copying them waits)
+        load_q(next);
+        locate(next.tile0 * DEC_TILE);
+        lookup((next.tile0 + 1) * DEC_TILE);
+        DEC_KEEP_LOADS();
+        load_k();
+        DEC_KEEP_LOADS();
+        load_v();
+        DEC_KEEP_LOADS();
+        if (worked) finish();
+        cur = next;
+        worked = true;
+        const int len = cur.len, heads = cur.heads, head0 = cur.head0;
         if constexpr (BIAS) {  // the weight of the unit's heads, by range
+            __syncthreads();  // (one wavefront: orders its LDS accesses)
             const int hb = heads > 1 ? 32 - __builtin_clz(heads - 1) : 0;
 #pragma unroll 4
             for (int i = lane; i < rel.n_ranges << hb; i += 64) {
@@ -277,13 +372,12 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
                             : rel.w_dtype == RGD_F16 ? to_f32(static_cast<const f16_t*>(rel.w)[at])
                                                      : to_f32(static_cast<const bf16_t*>(rel.w)[at]);
             }
-            __syncthreads();  // (one wavefront: orders its LDS accesses)
+            __syncthreads();
         }
 
-        f32x4 acc[VE];
 #pragma unroll
         for (int e = 0; e < VE; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float ref = -INFINITY, l = 0.f;
+        ref = -INFINITY, l = 0.f;
         const int hrow = min(n16, heads - 1);
 
         // one step; prefetch: the next one's keys are loaded as soon as this one's are used
@@ -304,6 +398,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
             if (prefetch) {
                 locate(t + DEC_TILE);
                 lookup(t + 2 * DEC_TILE);
+                DEC_KEEP_LOADS();
                 load_k();
             }
             float x8[8];
@@ -379,72 +474,39 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
             }
         };
 
+        const int t_last = (cur.tile1 - 1) * DEC_TILE;
         if (len > 0) {
-            locate(t0);
-            lookup(t0 + DEC_TILE);
-            load_k();
-            __builtin_amdgcn_sched_barrier(0);  // (keys before values here as in the loop: waits count loads in order)
-            load_v();
-            __builtin_amdgcn_sched_barrier(0);
-            const int t_last = (tile1 - 1) * DEC_TILE;
-            for (int t = t0; t < t_last; t += DEC_TILE) {
+            for (int t = cur.tile0 * DEC_TILE; t < t_last; t += DEC_TILE) {
                 ok_cur = ok_next;
                 step(t, true);
+                DEC_KEEP_LOADS();
                 load_v();
+                DEC_KEEP_LOADS();
             }
             ok_cur = ok_next;
-            step(t_last, false);
         }
-
-        // ---- the piece's result: lane holds channels VE m + e of head n16 for m = 4 g + r
-        l += xor_lanes(l, 16);
-        l += xor_lanes(l, 32);
-        const bool begins = tile0 == 0, ends = tile1 == ntiles;
-        if (begins && lane == 0) {
-            const int64_t last = base + (int64_t)unit * ntiles + ntiles - 1;
-            p.plan[(int64_t)b * p.units + unit] = make_int2((int)blockIdx.x, (int)(last <= INT32_MAX && share <= INT32_MAX ? (uint32_t)last / (uint32_t)share : last / share));
-        }
-        if (n16 < heads) {
-            if (begins && ends) {
-                const float inv = l == 0.f ? 0.f : 1.0f / l;
-                T* orow = static_cast<T*>(p.o) + b * p.so[0] + (int64_t)(head0 + n16) * p.so[1];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int first = (4 * g + r) * VE;
-                    T out[VE];
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) out[e] = from_f32<T>(l == 0.f ? 0.f : acc[e][r] * inv);
-                    if constexpr (SMALL) {
-#pragma unroll
-                        for (int e = 0; e < VE; ++e)
-                            if (first + e < D) orow[first + e] = out[e];
-                    } else {
-                        if (first < D) __builtin_memcpy(orow + min(first, D - VE), out, sizeof(out));
-                    }
-                }
-                if (p.lse && g == 0) p.lse[(int64_t)b * p.Hq + head0 + n16] = l == 0.f ? -INFINITY : (ref == -INFINITY ? 0.f : ref) + logf(l);
-            } else {
-                float* slot = p.part + (int64_t)(2 * blockIdx.x + (begins ? 1 : 0)) * ((int64_t)p.part_rows * DP + 32);
-                float out[4 * VE];
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) out[r * VE + e] = acc[e][r];
-                f32x4* to = reinterpret_cast<f32x4*>(slot + n16 * DP + 4 * g * VE);
-#pragma unroll
-                for (int i = 0; i < VE; ++i) to[i] = f32x4{out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]};
-                if (g == 0) {
-                    slot[p.part_rows * DP + n16] = ref;
-                    slot[p.part_rows * DP + 16 + n16] = l;
-                }
-            }
-        }
-        x += tile1 - tile0;
-        if (ends && unit + 1 == p.units) {
-            base += (int64_t)ntiles * p.units;
+        x += cur.tile1 - cur.tile0;
+        if (cur.tile1 == cur.ntiles && cur.unit + 1 == p.units) {
+            base += (int64_t)cur.ntiles * p.units;
             ++b;
         }
+        const bool more = x < x_end;
+        if (more) {
+            next = piece_at();
+            aim(next);
+            lookup(next.tile0 * DEC_TILE);
+        }
+        if (len > 0) step(t_last, false);
+        if (!more) break;
     }
+    finish();
+}
+
+// no page exists: every row is empty
+template <typename T> __global__ __launch_bounds__(64) void paged_decode_empty_kernel(const DecodeParams p) {
+    const int b = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
+    for (int d = threadIdx.x; d < p.D; d += 64) static_cast<T*>(p.o)[b * p.so[0] + (int64_t)h * p.so[1] + d] = from_f32<T>(0.f);
+    if (p.lse && threadIdx.x == 0) p.lse[(int64_t)b * p.Hq + h] = -INFINITY;
 }
 
 // One workgroup of THREADS per (sequence, query head): joins the pieces of its unit, in order.  32 lanes take 4 channels each, G
@@ -458,7 +520,8 @@ __global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(const Decod
     const int b = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
     const int hk = h / p.group, in_group = h - hk * p.group;
     const int unit = hk * p.head_tiles + (in_group >> 4), row = in_group & 15;
-    const int2 span = p.plan[(int64_t)b * p.units + unit];
+    const int* plan = &p.plan[2 * ((int64_t)b * p.units + unit)];
+    struct { int x, y; } span = {plan[0], plan[1]};
     if (span.x == span.y) return;  // one piece: written already
     const int64_t slot_size = (int64_t)p.part_rows * DP + 32;
     auto slot = [&](int w) { return p.part + (int64_t)(2 * w + (w == span.x ? 1 : 0)) * slot_size; };

@@ -5,16 +5,12 @@
 
 namespace {
 
-#ifndef DEC_WPS
-#define DEC_WPS 2
-#endif
-#ifndef DEC_LEAST
-#define DEC_LEAST 1
-#endif
-// Wavefronts of the decode launch
-int64_t decode_grid() { return (int64_t)rgd_num_cus() * 4 * DEC_WPS; }
-
 int chunks_of(int64_t D) { return (int)((D + 31) / 32); }
+// Wavefronts of the decode launch: those that are resident at once by their registers, three per SIMD for head dims up to 64, two
+// above.  More wait for their turn and leave more pieces to join, fewer leave loads in flight unused: at 1 / 2 / 3 per SIMD
+// (D = 64, 24 heads, 19 lengths to 2000) 44 / 35 / 33 us, (D = 128, 8 key heads, 64 lengths to 4100) 112 / 113 / 117 us,
+// (D = 128, 24 heads, 19 lengths to 2000) 58 / 54 / 57 us.
+int64_t decode_grid(int64_t D) { return (int64_t)rgd_num_cus() * 4 * (D <= 64 ? 3 : 2); }
 
 template <typename T, int NC, bool SMALL>
 int decode_launch(const DecodeParams& p, const DecodeBias* rel, unsigned grid, bool merge, hipStream_t s) {
@@ -46,8 +42,8 @@ extern "C" {
 size_t rgd_paged_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || D > 128) return 0;
     const int64_t group = Hq / Hkv, units = Hkv * ((group + 15) / 16), rows = group < 16 ? group : 16;
-    const int64_t plan = (B * units * (int64_t)sizeof(int2) + 15) / 16 * 16;
-    return (size_t)(plan + 2 * decode_grid() * (rows * 32 * chunks_of(D) + 32) * 4);
+    const int64_t plan = (B * units * 2 * (int64_t)sizeof(int) + 15) / 16 * 16;
+    return (size_t)(plan + 2 * decode_grid(D) * (rows * 32 * chunks_of(D) + 32) * 4);
 }
 
 int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_tensor4* q, const rgd_tensor4* k_cache,
@@ -117,16 +113,20 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
     p.num_pages = (int)num_pages;
     p.div_page = make_fastdiv((uint32_t)page_size);
     p.scale = softmax_scale;
-    p.least = DEC_LEAST;
     hipStream_t s = static_cast<hipStream_t>(stream);
     RGD_REQUIRE(workspace && workspace_bytes >= rgd_paged_decode_workspace(B, Hq, Hkv, D), RGD_ERR_WORKSPACE,
                 "%s: workspace of %zu bytes, needs %zu", name, workspace_bytes, rgd_paged_decode_workspace(B, Hq, Hkv, D));
-    p.plan = static_cast<int2*>(workspace);
-    p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (B * p.units * (int64_t)sizeof(int2) + 15) / 16 * 16);
+    p.plan = static_cast<int*>(workspace);
+    p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (B * p.units * 2 * (int64_t)sizeof(int) + 15) / 16 * 16);
+    if (none) {
+        const dim3 rows((unsigned)(B * Hq));
+        return rgd_launch_status(name, dtype == RGD_F16 ? rgd_launch(paged_decode_empty_kernel<f16_t>, rows, dim3(64), 0, s, p)
+                                                        : rgd_launch(paged_decode_empty_kernel<bf16_t>, rows, dim3(64), 0, s, p));
+    }
     // more wavefronts than there can be tiles have nothing to do; units of one tile are in no two wavefronts
     const int64_t most = p.capacity > DEC_TILE ? (p.capacity + DEC_TILE - 1) / DEC_TILE : 1;
     const int64_t tiles = B * p.units * most;
-    const unsigned grid = (unsigned)(tiles < decode_grid() ? tiles : decode_grid());
+    const unsigned grid = (unsigned)(tiles < decode_grid(D) ? tiles : decode_grid(D));
     return dtype == RGD_F16 ? decode_dispatch<f16_t>(p, bias, grid, most > 1, s) : decode_dispatch<bf16_t>(p, bias, grid, most > 1, s);
 }
 
