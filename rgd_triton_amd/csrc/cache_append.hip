@@ -185,8 +185,10 @@ int append_launch(AppendParams& p, int64_t B, int64_t tokens, bool ln, hipStream
     }
     p.blocks_q = blocks[0];
     p.blocks_k = blocks[1];
-    const dim3 grid(blocks[0] + blocks[1] + blocks[2]);
-    if (grid.x == 0) return RGD_OK;
+    const uint64_t all = (uint64_t)blocks[0] + blocks[1] + blocks[2];
+    if (all == 0) return RGD_OK;
+    RGD_REQUIRE(all < (1u << 24), RGD_ERR_UNSUPPORTED, "rgd_rope_cache_append: more rows than one launch takes");  // 2^32 threads
+    const dim3 grid((unsigned)all);
     const hipError_t e = ln ? rgd_launch(cache_append_kernel<T, TP, G, WIDE, true>, grid, dim3(256), 0, s, p)
                             : rgd_launch(cache_append_kernel<T, TP, G, WIDE, false>, grid, dim3(256), 0, s, p);
     return rgd_launch_status("rgd_rope_cache_append", e);

@@ -61,7 +61,7 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
     const int64_t lim = int64_t(1) << 31;
     RGD_REQUIRE(num_pages < lim && page_size < lim && max_pages < lim && max_pages * page_size <= lim - 1024, RGD_ERR_UNSUPPORTED,
                 "%s: more than 2^31 positions or pages", name);
-    RGD_REQUIRE(B < lim && Hq < lim && B * Hq < lim, RGD_ERR_UNSUPPORTED, "%s: more than 2^31 rows", name);
+    RGD_REQUIRE(B < lim && Hq < lim && B * Hq < (int64_t(1) << 24), RGD_ERR_UNSUPPORTED, "%s: 2^24 query rows or more", name);
     if (B == 0 || Hq == 0) return RGD_OK;
     RGD_REQUIRE(Hkv >= 1 && Hq % Hkv == 0, RGD_ERR_INVALID, "%s: query heads must be a multiple of the key heads", name);
     const bool none = num_pages == 0 || max_pages == 0;  // no key can exist

@@ -822,6 +822,7 @@ class Relative_Bias_Func(torch.autograd.Function):
         return _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, kernel_cache)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dbias):
         _no_capture("Relative_Bias_Func.backward")
         if ctx.kernel_cache is not None:
@@ -900,7 +901,7 @@ def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_tabl
     if torch.is_grad_enabled():
         _no_grad(what, query, key, value, pos_emb, k_cache, v_cache)
     head, tok = (1, 2) if heads_second else (2, 1)
-    shape, kshape, cache = query.shape, key.shape, k_cache.shape
+    shape, kshape, cshape = query.shape, key.shape, k_cache.shape
     index = query.get_device()
     dtype = query.dtype
     if not _seen(kernel_cache, "fwd", kernel_cache and _sig(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens) +
@@ -910,14 +911,14 @@ def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_tabl
         assert kshape == value.shape and kshape[0] == shape[0] and kshape[tok] == shape[tok] and kshape[3] == shape[3], \
             f"{query.shape=}, {key.shape=}, {value.shape=}"
         _check_cache(what, k_cache, v_cache, page_table, cache_lens, shape[0], dtype, shape[3])
-        assert cache[2] == kshape[head], f"{k_cache.shape=}, {key.shape=}"
+        assert cshape[2] == kshape[head], f"{k_cache.shape=}, {key.shape=}"
         if new_lens is not None:
             _check_lens(new_lens, shape[0])
         if pos_emb is not None:
             assert pos_emb.ndim == 3 and pos_emb.shape[0] == 2 and pos_emb.dtype in _FLOATS, f"{pos_emb.shape=}"
             assert pos_emb.shape[2] <= shape[3] and pos_emb.shape[2] % 2 == 0, f"{pos_emb.shape=}: an even rotary dim, at most {shape[3]}"
-            assert pos_emb.shape[1] >= page_table.shape[1] * cache[1], \
-                f"{pos_emb.shape=}: a row for every position of {page_table.shape[1]} pages of {cache[1]}"
+            assert pos_emb.shape[1] >= page_table.shape[1] * cshape[1], \
+                f"{pos_emb.shape=}: a row for every position of {page_table.shape[1]} pages of {cshape[1]}"
         _check_device(what, index, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens)
     if index != _current_device():
         with torch.cuda.device(index):
@@ -937,12 +938,14 @@ def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_tabl
         _desc4(query.data_ptr(), sq[0], sq[head], sq[tok]), _desc4(key.data_ptr(), sk[0], sk[head], sk[tok]),
         _desc4(value.data_ptr(), sv[0], sv[head], sv[tok]), _desc4(qo.data_ptr(), so[0], so[head], so[tok]),
         _desc4(k_cache.data_ptr(), ck_s[0], ck_s[2], ck_s[1]), _desc4(v_cache.data_ptr(), cv_s[0], cv_s[2], cv_s[1]),
-        cache[0], cache[1], page_table.data_ptr(), page_table.shape[1], page_table.stride(0), cache_lens.data_ptr(),
+        cshape[0], cshape[1], page_table.data_ptr(), page_table.shape[1], page_table.stride(0), cache_lens.data_ptr(),
         None if new_lens is None else new_lens.data_ptr(), *pe, cq, ck, norm_eps is not None, norm_eps or 0.0,
         _hip.dtype_code(dtype), _raw_stream(index))
     if rc:
         _hip.check(rc, "rgd_rope_cache_append")
-    torch.autograd.graph.increment_version((k_cache, v_cache))
+    for cache in (k_cache, v_cache):
+        if not cache.is_inference():  # (those have no version)
+            torch.autograd.graph.increment_version(cache)
     return qo
 
 

@@ -113,6 +113,7 @@ def test_append_refusals():
     assert _append(q=None) == -1 and _append(vc=None) == -1 and b"null tensor" in err()
     assert _append(size=1 << 20, per=1 << 12) == -2 and b"2^31" in err()
     assert _append(B=1 << 20, T=1 << 12) == -2
+    assert _append(B=1 << 14, T=1 << 14, Hq=2, Hkv=1) == -2 and b"one launch" in err()
     # nothing to do is no error
     assert _append(T=0) == 0 and _append(B=0) == 0 and _append(Hq=0, Hkv=0) == 0
 
@@ -128,6 +129,7 @@ def test_decode_refusals():
     assert _decode(lens=None) == -1 and _decode(table=None) == -1 and _decode(kc=None) == -1
     assert _decode(q=None) == -1 and _decode(o=None) == -1
     assert _decode(size=1 << 20, per=1 << 12) == -2
+    assert _decode(B=1 << 22, Hq=4) == -2 and b"query rows" in err()
     starts, buckets = (ctypes.c_int32 * 3)(-5, 0, 3), (ctypes.c_int32 * 3)(0, 1, 2)
     rel = dict(w=BUF, ws=4, nb=3, n=3, starts=starts, buckets=buckets)
     assert _decode(**{**rel, "wdt": 7}) == -1 and b"bias weights" in err()

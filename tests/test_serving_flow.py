@@ -170,3 +170,95 @@ def test_append_results_feed_decode_across_streams():
         o = layer.decode(qn, layer.k, layer.v, layer.pages, lens)
     ref = serving_oracle.decode(qn.cpu(), layer.k.cpu(), layer.v.cpu(), layer.pages.cpu(), lens.cpu(), 64**-0.5)
     check_decode(o, None, ref, 90, 64)
+
+
+def test_calls_in_inference_mode_and_from_threads():
+    """caches made in inference mode (they have no version counter), weights that require a gradient under no_grad, and two host
+    threads at once on streams of their own"""
+    import threading
+
+    import rgd_triton_amd as rgd
+
+    def work(seed, out):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream), torch.inference_mode():
+            layer = Layer(3, 4, 64, 16, 100, BF, True, 16, seed)
+            g = gen(seed + 1)
+            q, k, v = (randn(g, 3, 4, 60, 64, dtype=BF).cuda() for _ in range(3))
+            lens = torch.zeros(3, dtype=torch.int32, device="cuda")
+            got = [layer.append(q, k, v, layer.table, layer.k, layer.v, layer.pages, lens)]
+            lens += 60
+            for t in range(8):
+                got.append(layer.step(q[:, :, t:t + 1], k[:, :, t:t + 1], v[:, :, t:t + 1], lens))
+            got.append(layer.rel(40, 50, dtype=BF))
+        stream.synchronize()
+        out.append(got)
+
+    alone, together = [], []
+    for seed in (540, 550):
+        work(seed, alone)
+    errors = []
+
+    def guarded(seed, out):
+        try:
+            for _ in range(4):
+                work(seed, out)
+        except Exception as e:  # surfaced below
+            errors.append(repr(e))
+
+    lists = [[], []]
+    threads = [threading.Thread(target=guarded, args=(s, o)) for s, o in zip((540, 550), lists)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for want, outs in zip(alone, lists):
+        assert len(outs) == 4
+        for got in outs:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    w = torch.zeros(32, 4, device="cuda", requires_grad=True)
+    kc = torch.zeros(4, 16, 4, 64, device="cuda", dtype=BF)
+    args = (torch.zeros(1, 1, 4, 64, device="cuda", dtype=BF), kc, kc, torch.zeros(1, 4, device="cuda", dtype=torch.int32),
+            torch.ones(1, device="cuda", dtype=torch.int32))
+    with pytest.raises(AssertionError, match="no_grad"):
+        rgd.paged_decode_attn_func(*args, rel_weight=w)
+    with torch.no_grad():
+        assert (rgd.paged_decode_attn_func(*args, rel_weight=w) == 0).all()
+
+
+def test_bias_gradient_is_not_differentiated_twice():
+    from rgd_triton_amd import relative_position_bias_fn
+
+    w = torch.zeros(32, 2, device="cuda", requires_grad=True)
+    dy = torch.ones(1, 2, 30, 30, device="cuda", requires_grad=True)
+    (dw,) = torch.autograd.grad(relative_position_bias_fn(w, 30, 30), w, dy, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dw.sum(), dy)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,size,B,most", [(8, 1, 64, 16, 300, 90), (2, 2, 128, 8, 700, 40), (32, 2, 32, 1, 65, 70), (5, 5, 96, 48, 130, 33)])
+def test_many_short_sequences(Hq, Hkv, D, size, B, most):
+    """more sequences than one look at the lengths takes in (64), several units for each wavefront, empty ones among them; checked
+    against torch in 64 bits on the GPU"""
+    from rgd_triton_amd import paged_decode_attn_func
+
+    g = gen(560)
+    each = -(-most // size)
+    total = B * each + 1
+    pages = torch.randperm(total, generator=g)[: B * each].to(torch.int32).reshape(B, each)
+    lens = torch.randint(0, most + 1, (B,), generator=g, dtype=torch.int32)
+    lens[::7] = 0
+    q = randn(g, B, 1, Hq, D, dtype=BF).cuda()
+    k, v = (randn(g, total, size, Hkv, D, dtype=BF).cuda() for _ in range(2))
+    pages, lens = pages.cuda(), lens.cuda()
+    o, lse = paged_decode_attn_func(q, k, v, pages, lens, return_lse=True)
+    kk, vv = (c[pages.long()].reshape(B, each * size, Hkv, D).double().repeat_interleave(Hq // Hkv, 2).permute(0, 2, 1, 3).contiguous() for c in (k, v))
+    q64 = q.double().permute(0, 2, 1, 3)
+    s = (kk * q64).sum(-1) * D**-0.5
+    reach = (kk * q64).abs().sum(-1).amax(-1) * D**-0.5
+    seen = torch.arange(each * size, device="cuda") < lens[:, None]
+    s = s.masked_fill(~seen[:, None], float("-inf"))
+    p = torch.softmax(s, -1).nan_to_num(0.0)
+    ref = ((p[..., None] * vv).sum(2)[:, None], torch.logsumexp(s, -1), (p[..., None] * vv.abs()).sum(2)[:, None], reach)
+    check_decode(o, lse, tuple(t.cpu() for t in ref), most, D)
