@@ -326,7 +326,8 @@ int rgd_attn_bwd(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t D,
  * rot as in rgd_rope_qk with the table row of the position (channels < R of positions < q_cutoff / k_cutoff; R even),
  * norm the LayerNorm over D without affine when layer_norm != 0, else nothing.  R > 0 needs P >= max_pages * page_size.
  * Cache rows of no new token are left as they were.  cache_lens itself is not changed.  Two tokens of one call must not fall
- * on the same slot (a page that stands twice in the table; what the slot then holds is undefined).  qo may be q. */
+ * on the same slot (a page that stands twice in the table; what the slot then holds is undefined), nor the caches share memory.
+ * qo may be q.  Fewer than 2^24 workgroups of 256 threads in all (2^24 x 16 row pairs at D > 64). */
 int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                           const rgd_tensor4* q, const rgd_tensor4* k, const rgd_tensor4* v, const rgd_tensor4* qo,
                           const rgd_tensor4* k_cache, const rgd_tensor4* v_cache, int64_t num_pages, int64_t page_size,
@@ -342,7 +343,7 @@ int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t
  * rel_weight (NULL: no bias): bias_j = weight[bucket * w_stride + h] of the range (see rgd_rel_bias_fwd) that holds
  * j - (seq_lens[b] - 1); starts and buckets are HOST arrays, read during the call.
  * Statistics and sums are fp32; every result is reproducible bit for bit.  Calls that may overlap in time need separate
- * workspaces (any contents on entry, 16-byte aligned). */
+ * workspaces (any contents on entry, 16-byte aligned).  B * Hq below 2^24. */
 size_t rgd_paged_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
 int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_tensor4* q,
                      const rgd_tensor4* k_cache, const rgd_tensor4* v_cache, int64_t num_pages, int64_t page_size,
@@ -358,7 +359,8 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
  *   bias[h, i, j] = weight[bucket(d) * w_stride + h],  d = j - i - q_offset
  * Buckets are ranges of d: range k < n_ranges holds starts[k] <= d < starts[k + 1] and has bucket buckets[k]; range 0 holds
  * everything below starts[1] (starts[0] is not read) and the last one everything from its start on.  Starts ascend and
- * no bucket has two ranges; starts and buckets are HOST arrays, read during the call; at most 256 ranges and buckets.
+ * no bucket has two ranges; starts and buckets are HOST arrays, read during the call; at most 256 ranges and buckets.  Sizes
+ * and q_offset stay below 2^30, Tq + Tk + |q_offset| at most 2^31 - 2048, H at most 65535.
  * ------------------------------------------------------------------------------------------ */
 
 /* bias by (head, row) strides (stride_h, stride_n), any dtype.  Scratch (any contents on entry, 16-byte aligned; 0 bytes for

@@ -33,7 +33,7 @@ struct AppendRows {  // one of q, k, v
 struct AppendParams {
     AppendRows t[3];
     uint32_t blocks_q, blocks_k;  // row blocks of q, then of k, then of v
-    int D, T, R;
+    int D, R;
     float inv_d, eps;
     const int32_t* page_table;
     const int32_t* cache_lens;
@@ -252,7 +252,6 @@ extern "C" int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t H
         a.cutoff = (int)(cutoff < 0 ? 0 : (cutoff < lim - 1 ? cutoff : lim - 1));
     }
     p.D = (int)D;
-    p.T = (int)T;
     p.R = (int)R;
     p.inv_d = 1.0f / (float)D;
     p.eps = eps;

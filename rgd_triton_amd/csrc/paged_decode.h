@@ -50,7 +50,7 @@ struct DecodeParams {
     const int32_t* seq_lens;
     int64_t table_stride;
     int32_t capacity;  // positions of a page table row
-    int B, Hq, Hkv, group, head_tiles, units;  // units = Hkv * head_tiles, per sequence
+    int B, Hq, group, head_tiles, units;  // units = key heads * head_tiles, per sequence
     int D, num_pages;
     FastDiv div_page;
     float scale;
@@ -96,12 +96,6 @@ template <int N> __device__ __forceinline__ void stream_dwords(const char* p, ui
 #pragma unroll
         for (int i = 0; i < N; ++i) out[i] = v[i];
     }
-}
-
-// a value that is the same in all lanes, for the scalar unit
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
-    return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
 __device__ __forceinline__ float xor_lanes(float v, int m) { return __shfl_xor(v, m, 64); }

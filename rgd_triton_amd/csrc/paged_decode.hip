@@ -77,6 +77,7 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
         RGD_REQUIRE(n_ranges >= 1 && n_ranges <= DEC_MAX_RANGES && starts && buckets, RGD_ERR_INVALID, "%s: 1 to %d ranges", name, DEC_MAX_RANGES);
         for (int64_t i = 0; i < n_ranges; ++i) {
             RGD_REQUIRE(buckets[i] >= 0 && buckets[i] < num_buckets, RGD_ERR_INVALID, "%s: a bucket outside the weight", name);
+            RGD_REQUIRE(i < 2 || starts[i] > starts[i - 1], RGD_ERR_INVALID, "%s: range starts must ascend", name);
             rel.start[i] = starts[i];
             rel.bucket[i] = buckets[i];
         }
@@ -103,11 +104,10 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
     p.table_stride = table_stride;
     p.capacity = none ? 0 : (int)(max_pages * page_size);
     p.B = (int)B;
-    p.Hkv = (int)Hkv;
     p.Hq = (int)Hq;
     p.group = (int)(Hq / Hkv);
     p.head_tiles = (p.group + 15) / 16;
-    p.units = p.Hkv * p.head_tiles;
+    p.units = (int)Hkv * p.head_tiles;
     p.part_rows = p.group < 16 ? p.group : 16;
     p.D = (int)D;
     p.num_pages = (int)num_pages;

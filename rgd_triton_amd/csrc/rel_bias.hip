@@ -6,8 +6,8 @@
 // is the sum of each diagonal, added up over the diagonals of a bucket.  Bound by memory: the matrix is written (forward) or
 // read (backward) once.
 //
-// The backward, and the forward of a matrix that fits the Infinity Cache, walk the matrix along its diagonals.  A wavefront takes a
-// strip of 512 columns and goes down `chunk` rows, 8 rows and 8 columns at a time: lane l holds the 8 x 8 block whose columns
+// The backward, and the forward of a matrix of up to 64 MB, walk the matrix along its diagonals.  A wavefront takes a strip of 512
+// columns and goes down `chunk` rows, 8 rows and 8 columns at a time: lane l holds the 8 x 8 block whose columns
 // begin at strip + 8 l + 8 n in step n, so the 15 diagonals of a lane's block are the same in every step.
 //   forward   the 15 values are looked up once, the 8 rows of the block packed once; each step is eight 16-byte stores
 //   backward  15 sums stay in registers; each step is eight 16-byte streaming loads and 64 additions
@@ -345,6 +345,7 @@ int check_shape(const char* name, int64_t H, int64_t Tq, int64_t Tk, int64_t num
     RGD_REQUIRE(H <= 65535, RGD_ERR_UNSUPPORTED, "%s: more than 65535 heads", name);
     const int64_t lim = int64_t(1) << 30;
     RGD_REQUIRE(Tq < lim && Tk < lim && offset > -lim && offset < lim, RGD_ERR_UNSUPPORTED, "%s: positions beyond 2^30", name);
+    RGD_REQUIRE(Tq + Tk + (offset < 0 ? -offset : offset) <= 2 * lim - 2048, RGD_ERR_UNSUPPORTED, "%s: distances beyond 2^31", name);
     RGD_REQUIRE(n_ranges >= 1 && n_ranges <= MAX_RANGES && num_buckets >= 1 && num_buckets <= MAX_RANGES && starts && buckets,
                 RGD_ERR_INVALID, "%s: 1 to %d ranges and buckets", name, MAX_RANGES);
     bool used[MAX_RANGES] = {};

@@ -893,7 +893,8 @@ def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_tabl
     stored, query rows zero).  pos_emb as in triton_rope_fn, with a row for every position the page table covers; None: no
     rotation.  Positions from seq_cutoff on (an int, or one for query and one for key) are not rotated.  norm_eps: LayerNorm over
     the head dim in front of the rotation, as triton_fused_ln_rope_fn has it; None: none.  A token whose page number is outside
-    the cache is not stored; one whose position is outside the page table is padding.  cache_lens is the caller's to advance."""
+    the cache is not stored; one whose position is outside the page table is padding.  Two tokens of a call must not fall on one slot
+    (a page twice in the table), and the two caches must not share memory.  cache_lens is the caller's to advance."""
     what = "rope_cache_append"
     query, key, value = _lastdim_contig(query, key, value)
     if pos_emb is not None:
@@ -1000,7 +1001,7 @@ def paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight
         B, Hq, cache[2], D, _desc4(q.data_ptr(), sq[0], sq[2], sq[1]), _desc4(k_cache.data_ptr(), ck_s[0], ck_s[2], ck_s[1]),
         _desc4(v_cache.data_ptr(), cv_s[0], cv_s[2], cv_s[1]), cache[0], cache[1], page_table.data_ptr(), page_table.shape[1],
         page_table.stride(0), seq_lens.data_ptr(), *rel, _desc4(o.data_ptr(), Hq * D, D, 0), None if lse is None else lse.data_ptr(),
-        _hip.dtype_code(dtype), softmax_scale or 1.0 / math.sqrt(D), ws.data_ptr(), nbytes, _raw_stream(index))
+        _hip.dtype_code(dtype), 1.0 / math.sqrt(D) if softmax_scale is None else softmax_scale, ws.data_ptr(), nbytes, _raw_stream(index))
     if rc:
         _hip.check(rc, "rgd_paged_decode")
     return (o, lse) if return_lse else o

@@ -135,6 +135,7 @@ def test_decode_refusals():
     assert _decode(**{**rel, "wdt": 7}) == -1 and b"bias weights" in err()
     assert _decode(**{**rel, "nb": 2}) == -1 and b"bucket outside" in err()
     assert _decode(**{**rel, "n": 0}) == -1 and _decode(**{**rel, "n": 257}) == -1 and _decode(**{**rel, "starts": None}) == -1
+    assert _decode(**{**rel, "starts": (ctypes.c_int32 * 3)(-5, 3, 0)}) == -1 and b"ascend" in err()
     need = _hip.lib().rgd_paged_decode_workspace(1, 4, 2, 64)
     assert need > 0 and _decode(bytes=need - 1) == -4 and b"workspace" in err() and _decode(work=None) == -4
     assert _decode(B=0) == 0 and _decode(Hq=0, Hkv=1) == 0
@@ -159,6 +160,7 @@ def test_rel_bias_refusals():
     for f in (fwd, bwd):
         assert f(wdt=3) == -1 and b"Only support" in err()
         assert f(Tq=-1) == -1 and f(H=70000) == -2 and f(Tk=1 << 30) == -2 and f(off=1 << 30) == -2 and f(off=-(1 << 30)) == -2
+        assert f(Tq=1 << 29, Tk=1 << 29, off=(1 << 30) - 1) == -2 and b"distances" in err()
         assert f(n=0) == -1 and f(n=257) == -1 and f(nb=257) == -1 and f(starts=None) == -1
         assert f(starts=down) == -1 and b"ascend" in err()
         assert f(buckets=twice) == -1 and b"two ranges" in err()

@@ -1,5 +1,7 @@
 """The operators as they are used together: a prompt is appended to the cache, then every new token is appended and attends over
 it, eagerly and from a replayed graph; and the same sequence through RoPE and FlashAttention as a whole."""
+import math
+
 import pytest
 import torch
 
@@ -262,3 +264,18 @@ def test_many_short_sequences(Hq, Hkv, D, size, B, most):
     p = torch.softmax(s, -1).nan_to_num(0.0)
     ref = ((p[..., None] * vv).sum(2)[:, None], torch.logsumexp(s, -1), (p[..., None] * vv.abs()).sum(2)[:, None], reach)
     check_decode(o, lse, tuple(t.cpu() for t in ref), most, D)
+
+
+def test_decode_softmax_scale_of_zero_is_the_mean():
+    """scale 0 is a scale, not the default: every key weighs the same"""
+    from rgd_triton_amd import paged_decode_attn_func
+
+    g = gen(570)
+    q, k, v = randn(g, 1, 1, 4, 64, dtype=BF).cuda(), randn(g, 5, 16, 2, 64, dtype=BF).cuda(), randn(g, 5, 16, 2, 64, dtype=BF).cuda()
+    pages = torch.tensor([[3, 0, 4, 1]], dtype=torch.int32, device="cuda")
+    o, lse = paged_decode_attn_func(q, k, v, pages, torch.tensor([55], dtype=torch.int32, device="cuda"), softmax_scale=0.0, return_lse=True)
+    vv = v[pages[0].long()].reshape(64, 2, 64)[:55].double()
+    ref, mag = (t.mean(0).repeat_interleave(2, 0) for t in (vv, vv.abs()))
+    # one rounding to bf16 (2^-8), the probabilities' parts 2^-14, fp32 sums
+    assert ((o[0, 0].double() - ref).abs() <= 2**-8 * ref.abs() + 2**-13 * mag).all()
+    assert (lse.double() - math.log(55)).abs().max() <= 2**-20
