@@ -27,7 +27,7 @@
 //
 // Measured (this launch / the merge; a read that streams 512 MB reaches 6.6 TB/s): one sequence of 131000 keys, 32 / 8 heads,
 // D = 128: 86 / 7 us, 6.2 TB/s; 64 sequences to 4100 keys, the same heads: 106 / 5 us, 5.5 TB/s; 19 to 2000 keys, 24 heads,
-// D = 80, bias, pages of 5: 53 / 5 us; one of 200 keys, 16 heads, D = 64: 5.8 / 3.5 us.  What a launch takes beyond its
+// D = 80, bias, pages of 5: 45 / 5 us; one of 200 keys, 16 heads, D = 64: 5.3 / 3.6 us.  What a launch takes beyond its
 // bytes, about 15 us, is the chain of loads in front of the first step (lengths, page numbers, keys), the last steps, in which
 // the wavefronts run out one by one, and the merge.
 #pragma once
@@ -38,6 +38,7 @@
 
 constexpr int DEC_MAX_RANGES = 256;
 constexpr int DEC_TILE = 32;  // keys of a step
+constexpr int DEC_NEAR = 256;  // distances whose range is looked up instead of searched
 
 struct DecodeParams {
     const void* q;
@@ -65,6 +66,7 @@ struct DecodeBias {  // relative bias: weight (buckets, Hq), ranges of the dista
     int w_dtype, n_ranges;
     int half;  // largest power of two below n_ranges (0 for one range)
     int start[DEC_MAX_RANGES], bucket[DEC_MAX_RANGES];
+    uint32_t near[DEC_NEAR / 4];  // bytes: range of the distance -n, n < DEC_NEAR
 };
 struct DecodeNoBias {};  // (2 KB less to hand over with every launch)
 
@@ -80,19 +82,18 @@ template <> struct Mfma16<f16_t> {
     }
 };
 
-// N dwords from an address of any alignment (the hardware takes unaligned vector loads; rows of an odd head dim need them)
-template <int N> __device__ __forceinline__ void load_dwords(const char* p, uint32_t (&out)[N]) {
-    __builtin_memcpy(out, p, 4 * N);
-}
-// streaming: a key or value is read once
-template <int N> __device__ __forceinline__ void stream_dwords(const char* p, uint32_t (&out)[N]) {
+// N dwords from an address of any alignment (the hardware takes unaligned vector loads; rows of an odd head dim need them); NT:
+// streaming
+template <int N, bool NT = false> __device__ __forceinline__ void load_dwords(const char* p, uint32_t (&out)[N]) {
     if constexpr (N == 1) {
         typedef uint32_t V __attribute__((aligned(2)));
-        out[0] = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+        const V* from = reinterpret_cast<const V*>(p);
+        out[0] = NT ? __builtin_nontemporal_load(from) : *from;
     } else {
         typedef uint32_t V0 __attribute__((ext_vector_type(N)));
         typedef V0 V __attribute__((aligned(2)));
-        const V0 v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+        const V* from = reinterpret_cast<const V*>(p);
+        const V0 v = NT ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
         for (int i = 0; i < N; ++i) out[i] = v[i];
     }
@@ -122,9 +123,19 @@ template <typename T, int NC, bool SMALL, bool BIAS>
 __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams p,
                                                           const std::conditional_t<BIAS, DecodeBias, DecodeNoBias> rel) {
     constexpr int DP = 32 * NC, VE = DP / 16, VW = VE / 2;
-    __shared__ int s_start[BIAS ? DEC_MAX_RANGES : 1], s_bucket[BIAS ? DEC_MAX_RANGES : 1];
-    __shared__ float s_w[BIAS ? DEC_MAX_RANGES : 1][16];
+    // Where rows of token-major heads fill whole 128-byte lines (D = 64, 128) no other wavefront reads a line: loads stream.  Else
+    // neighbouring heads share lines and they do not; and where a line holds whole rows of several heads, neighbouring runs go
+    // to one XCD, whose L2 then has them.  Streaming / not / not and by XCD: (19 x 24 heads, lengths to 2000) D = 16: 28 / 27 /
+    // 20 us, D = 32: 28 / 28 / 24, D = 80: 47 / 44 / 44; one of 131000 keys, 8 key heads, D = 80: 94 / 82 / 88, D = 128: 95 / 104 / 111.
+    constexpr bool ALONE = NC % 2 == 0, BY_XCD = NC == 1;
+    // BIAS, by the number of ranges (for 256 of them 8 wavefronts fit a compute unit, for 32 all 12 of the small head dims do:
+    // D = 64, 24 heads, 19 lengths to 2000 with bias 37 us instead of 42)
+    static_assert(DEC_NEAR == 4 * 64, "a dword per lane");
+    extern __shared__ uint32_t s_near[];  // then starts, buckets and the weight of 16 heads
+    int *s_start = nullptr, *s_bucket = nullptr;
+    float (*s_w)[16] = nullptr;
 
+    const int wave = BY_XCD && gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
     const int lane = threadIdx.x;
     const int n16 = lane & 15, g = lane >> 4;
     const int D = p.D;
@@ -135,7 +146,12 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
     auto tiles_of = [](int len) { return len > 0 ? (int)(((uint32_t)len + DEC_TILE - 1) / DEC_TILE) : 1; };
 
     if constexpr (BIAS) {  // (starts filled up to the next power of two: a search halves it)
-        for (int r = lane; r < DEC_MAX_RANGES; r += 64) {
+        const int fill = max(2 * rel.half, 1);
+        s_start = reinterpret_cast<int*>(s_near + DEC_NEAR / 4);
+        s_bucket = s_start + fill;
+        s_w = reinterpret_cast<float(*)[16]>(s_bucket + fill);
+        s_near[lane] = rel.near[lane];
+        for (int r = lane; r < fill; r += 64) {
             s_start[r] = r < rel.n_ranges ? (r == 0 ? INT32_MIN : rel.start[r]) : INT32_MAX;
             s_bucket[r] = r < rel.n_ranges ? rel.bucket[r] : 0;
         }
@@ -158,8 +174,8 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
     for (int b0 = 64; b0 < p.B; b0 += 64) total += last_of(scan(b0 + lane < p.B ? tiles_of(length(b0 + lane)) : 0));
     total *= p.units;
     const int64_t even = total <= INT32_MAX ? (int64_t)((uint32_t)total / gridDim.x) : total / gridDim.x, rest = total - even * gridDim.x;
-    int64_t x = even * blockIdx.x + min((int64_t)blockIdx.x, rest);
-    const int64_t x_end = x + even + (blockIdx.x < rest ? 1 : 0);
+    int64_t x = even * wave + min((int64_t)wave, rest);
+    const int64_t x_end = x + even + (wave < rest ? 1 : 0);
     if (x >= x_end) return;
     int b = 0;
     int64_t base = 0;  // first tile of sequence b
@@ -248,7 +264,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
                     kf[a][c] = r.v;
                 } else {
                     uint32_t r[4];
-                    stream_dwords<4>(reinterpret_cast<const char*>(row + kstart[c]), r);
+                    load_dwords<4, ALONE>(reinterpret_cast<const char*>(row + kstart[c]), r);
                     kf[a][c] = u32x4{r[0], r[1], r[2], r[3]};
                 }
             }
@@ -262,7 +278,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
                 const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
                 vr[i][0] = r[min(vstart, D - 1)] | (uint32_t)r[min(vstart + 1, D - 1)] << 16;
             } else {
-                stream_dwords<VW>(reinterpret_cast<const char*>(row + vstart), vr[i]);
+                load_dwords<VW, ALONE>(reinterpret_cast<const char*>(row + vstart), vr[i]);
             }
         }
     };
@@ -302,8 +318,8 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
         l += xor_lanes(l, 32);
         if (lane == 0) {
             int* plan = &p.plan[2 * ((int64_t)cur.b * p.units + cur.unit)];
-            if (begins) plan[0] = (int)blockIdx.x;
-            if (ends) plan[1] = (int)blockIdx.x;
+            if (begins) plan[0] = wave;
+            if (ends) plan[1] = wave;
         }
         if (n16 < heads) {
             if (begins && ends) {
@@ -325,7 +341,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
                 }
                 if (p.lse && g == 0) p.lse[(int64_t)cur.b * p.Hq + head0 + n16] = l == 0.f ? -INFINITY : (ref == -INFINITY ? 0.f : ref) + logf(l);
             } else {
-                float* slot = p.part + (int64_t)(2 * blockIdx.x + (begins ? 1 : 0)) * ((int64_t)p.part_rows * DP + 32);
+                float* slot = p.part + (int64_t)(2 * wave + (begins ? 1 : 0)) * ((int64_t)p.part_rows * DP + 32);
                 float out[4 * VE];
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
@@ -404,6 +420,10 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
                     const float wv = s_w[0][hrow];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x8[i] += wv;
+                } else if (len - t <= DEC_NEAR) {  // (searched, (19 x 24 heads, lengths to 2000) D = 128 takes 58 us instead of 54)
+                    const uint8_t* near = reinterpret_cast<const uint8_t*>(s_near);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x8[i] += s_w[near[max(-d0 - i, 0)]][hrow];
                 } else {
                     int at[8];  // last range that begins at or before the key's distance, the 8 searches side by side
 #pragma unroll

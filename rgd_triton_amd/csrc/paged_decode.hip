@@ -14,7 +14,8 @@ int64_t decode_grid(int64_t D) { return (int64_t)rgd_num_cus() * 4 * (D <= 64 ? 
 
 template <typename T, int NC, bool SMALL>
 int decode_launch(const DecodeParams& p, const DecodeBias* rel, unsigned grid, bool merge, hipStream_t s) {
-    const hipError_t e = rel ? rgd_launch(paged_decode_kernel<T, NC, SMALL, true>, dim3(grid), dim3(64), 0, s, p, *rel)
+    const size_t lds = rel ? DEC_NEAR + (rel->half ? 2 * rel->half : 1) * 2 * sizeof(int) + rel->n_ranges * 16 * sizeof(float) : 0;
+    const hipError_t e = rel ? rgd_launch(paged_decode_kernel<T, NC, SMALL, true>, dim3(grid), dim3(64), lds, s, p, *rel)
                              : rgd_launch(paged_decode_kernel<T, NC, SMALL, false>, dim3(grid), dim3(64), 0, s, p, DecodeNoBias{});
     const int rc = rgd_launch_status("rgd_paged_decode", e);
     if (rc != RGD_OK || !merge) return rc;
@@ -86,6 +87,12 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
         rel.w_dtype = w_dtype;
         rel.n_ranges = (int)n_ranges;
         for (rel.half = 0; (rel.half ? 2 * rel.half : 1) < n_ranges;) rel.half = rel.half ? 2 * rel.half : 1;
+        uint8_t near[DEC_NEAR];
+        for (int n = 0, r = rel.n_ranges - 1; n < DEC_NEAR; ++n) {
+            for (; r > 0 && rel.start[r] > -n;) --r;
+            near[n] = (uint8_t)r;
+        }
+        memcpy(rel.near, near, sizeof(near));
         bias = &rel;
     }
     p.q = q->ptr;
