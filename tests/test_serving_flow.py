@@ -279,3 +279,38 @@ def test_decode_softmax_scale_of_zero_is_the_mean():
     # one rounding to bf16 (2^-8), the probabilities' parts 2^-14, fp32 sums
     assert ((o[0, 0].double() - ref).abs() <= 2**-8 * ref.abs() + 2**-13 * mag).all()
     assert (lse.double() - math.log(55)).abs().max() <= 2**-20
+
+
+def test_padded_prompt_rotated_beforehand_then_a_token():
+    """a prompt through RoPE and FlashAttention, stored as it is rotated (no table), then a token: the cache holds RoPE's keys bit
+    for bit, padding and foreign slots stay as they were, and the token sees its sequence"""
+    import rgd_triton_amd as rgd
+
+    B, H, T, D, size = 3, 4, 37, 64, 8
+    layer = Layer(B, H, D, size, 48, BF, False, 0, 580)
+    g = gen(581)
+    q, k, v = (randn(g, B, H, T, D, dtype=BF).cuda() for _ in range(3))
+    q1, k1, v1 = (randn(g, B, H, 1, D, dtype=BF).cuda() for _ in range(3))
+    plens = torch.tensor([37, 0, 16], dtype=torch.int32, device="cuda")
+    lens = torch.zeros(B, dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        q, k = rgd.RoPE()(q, k, layer.table)
+        out = layer.append(q, k, v, None, layer.k, layer.v, layer.pages, lens, new_lens=plens)
+        lens += plens
+        kc = layer.k.clone()
+        o = layer.step(q1, k1, v1, lens)
+    written = torch.zeros(kc.shape[:2], dtype=torch.bool, device="cuda")
+    for b in range(B):
+        n = int(plens[b])
+        assert torch.equal(out[b, :, :n], q[b, :, :n]) and (out[b, :, n:] == 0).all()
+        for j in range(n):
+            page, slot = int(layer.pages[b, j // size]), j % size
+            written[page, slot] = True
+            assert torch.equal(kc[page, slot], k[b, :, j])
+    assert kc[~written].isnan().all()
+    assert lens.tolist() == [38, 1, 17]
+    assert torch.equal(o[1, 0], v1[1, :, 0])  # its own key is all it sees
+    ref = serving_oracle.decode(rgd.RoPE()(q1, k1, layer.table[:, 37:39].contiguous())[0][:1].transpose(1, 2).cpu(), layer.k.cpu(), layer.v.cpu(),
+                                layer.pages[:1].cpu(), lens[:1].cpu(), D**-0.5, None, 0, False)[0]
+    # the query's rotation is rounded by two kernels (half a step each way) in front of the logits
+    assert (o[:1].double().cpu() - ref).abs().max() <= 16 * half_step(BF) * v.double().abs().max().item()
