@@ -328,14 +328,20 @@ int rgd_attn_bwd(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t D,
  * Cache rows of no new token are left as they were.  cache_lens itself is not changed.  Two tokens of one call must not fall
  * on the same slot (a page that stands twice in the table; what the slot then holds is undefined), nor the caches share memory.
  * qo may be q.  Fewer than 2^24 workgroups of 256 threads in all (2^24 x 16 row pairs at D > 64). */
-int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
-                          const rgd_tensor4* q, const rgd_tensor4* k, const rgd_tensor4* v, const rgd_tensor4* qo,
-                          const rgd_tensor4* k_cache, const rgd_tensor4* v_cache, int64_t num_pages, int64_t page_size,
-                          const int32_t* page_table, int64_t max_pages, int64_t table_stride,
-                          const int32_t* cache_lens, const int32_t* new_lens,
-                          const void* pos_emb, int64_t P, int64_t R, int64_t pe_stride_s, int64_t pe_stride_n,
-                          int pe_dtype, int64_t q_cutoff, int64_t k_cutoff, int layer_norm, float eps,
-                          int dtype, void* stream);
+typedef struct rgd_cache_append_args { /* one structure: a call per token and layer, whose host time counts */
+    int64_t B, T, Hq, Hkv, D;
+    rgd_tensor4 q, k, v, qo, k_cache, v_cache;
+    int64_t num_pages, page_size;
+    const int32_t* page_table;
+    int64_t max_pages, table_stride;
+    const int32_t* cache_lens;
+    const int32_t* new_lens;
+    const void* pos_emb;
+    int64_t P, R, pe_stride_s, pe_stride_n, q_cutoff, k_cutoff;
+    int32_t pe_dtype, layer_norm, dtype;
+    float eps;
+} rgd_cache_append_args;
+int rgd_rope_cache_append(const rgd_cache_append_args* args, void* stream);
 
 /* o[b, h] = sum_j softmax_j(softmax_scale q[b, h] . k_j + bias_j) v_j over the positions j < seq_lens[b] (the new token's
  * own key is among them), h reading key head h / (Hq / Hkv).  q and o use stride_b and stride_h.  lse (NULL or fp32 (B, Hq))
@@ -345,13 +351,24 @@ int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t
  * Statistics and sums are fp32; every result is reproducible bit for bit.  Calls that may overlap in time need separate
  * workspaces (any contents on entry, 16-byte aligned).  B * Hq below 2^24. */
 size_t rgd_paged_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
-int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_tensor4* q,
-                     const rgd_tensor4* k_cache, const rgd_tensor4* v_cache, int64_t num_pages, int64_t page_size,
-                     const int32_t* page_table, int64_t max_pages, int64_t table_stride, const int32_t* seq_lens,
-                     const void* rel_weight, int64_t w_stride, int64_t num_buckets, int w_dtype,
-                     int64_t n_ranges, const int32_t* starts, const int32_t* buckets,
-                     const rgd_tensor4* o, float* lse, int dtype, float softmax_scale,
-                     void* workspace, size_t workspace_bytes, void* stream);
+typedef struct rgd_paged_decode_args {
+    int64_t B, Hq, Hkv, D;
+    rgd_tensor4 q, k_cache, v_cache, o;
+    int64_t num_pages, page_size;
+    const int32_t* page_table;
+    int64_t max_pages, table_stride;
+    const int32_t* seq_lens;
+    const void* rel_weight;
+    int64_t w_stride, num_buckets, n_ranges;
+    const int32_t* starts;
+    const int32_t* buckets;
+    float* lse;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t w_dtype, dtype;
+    float softmax_scale;
+} rgd_paged_decode_args;
+int rgd_paged_decode(const rgd_paged_decode_args* args, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Learned relative position bias, an attention bias (1, H, Tq, Tk) from a weight (num_buckets, H).  No counterpart in

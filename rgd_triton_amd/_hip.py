@@ -38,7 +38,8 @@ _i64, _int, _f32, _vp, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctype
 _T3, _T4 = ctypes.POINTER(Tensor3), ctypes.POINTER(Tensor4)
 
 # argument types of every entry point, in the order of include/rgd_hip.h (the operators that a serving loop calls token by
-# token take their tensor descriptors as packed bytes, see desc4: half of the host time of building and converting structures)
+# token, and the learned bias, take descriptors or all their arguments as packed bytes, see below: building and converting
+# them one by one was half of a call's host time)
 _SIGNATURES = {
     "rgd_version": (_int, []),
     "rgd_last_error": (ctypes.c_char_p, []),
@@ -70,11 +71,9 @@ _SIGNATURES = {
     "rgd_attn_bwd_workspace": (_sz, [_i64] * 5 + [_int]),
     "rgd_attn_bwd": (_int, [_i64] * 5 + [_T4] * 5 + [_vp] + [_T4, _int, _int] + [_T4] * 4 + [_int, _int, _f32, _int, _vp,
                                                                                          _vp, _sz, _vp]),
-    "rgd_rope_cache_append": (_int, [_i64] * 5 + [_vp] * 6 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp] + [_i64] * 4 +
-                              [_int, _i64, _i64, _int, _f32, _int, _vp]),
+    "rgd_rope_cache_append": (_int, [_vp, _vp]),
     "rgd_paged_decode_workspace": (_sz, [_i64] * 4),
-    "rgd_paged_decode": (_int, [_i64] * 4 + [_vp] * 3 + [_i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, _i64, _vp, _vp,
-                                                         _vp, _vp, _int, _f32, _vp, _sz, _vp]),
+    "rgd_paged_decode": (_int, [_vp, _vp]),
     "rgd_rel_bias_fwd_workspace": (_sz, [_i64] * 3 + [_int]),
     "rgd_rel_bias_fwd": (_int, [_i64] * 3 + [_vp, _i64, _i64, _int, _i64, _vp, _vp, _i64, _vp, _int, _vp, _sz, _vp]),
     "rgd_rel_bias_bwd_workspace": (_sz, [_i64] * 4),
@@ -149,6 +148,9 @@ def t4(t, heads_second):
 
 # an rgd_tensor4 as bytes, accepted where an entry point's argument is declared void*: (pointer, stride_b, stride_h, stride_n)
 desc4 = struct.Struct("@Pqqq").pack
+# rgd_cache_append_args and rgd_paged_decode_args, member by member in the header's order (0 for a null pointer)
+append_args = struct.Struct("@5q" + "Pqqq" * 6 + "2qP2q3P6q3if").pack
+decode_args = struct.Struct("@4q" + "Pqqq" * 4 + "2qP2q2P3q4PN2if4x").pack
 
 
 def stream_ptr(device):

@@ -203,14 +203,12 @@ template <typename T, typename TP> int append_dispatch(AppendParams& p, int64_t 
 
 }  // namespace
 
-extern "C" int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, const rgd_tensor4* q,
-                                     const rgd_tensor4* k, const rgd_tensor4* v, const rgd_tensor4* qo,
-                                     const rgd_tensor4* k_cache, const rgd_tensor4* v_cache, int64_t num_pages,
-                                     int64_t page_size, const int32_t* page_table, int64_t max_pages, int64_t table_stride,
-                                     const int32_t* cache_lens, const int32_t* new_lens, const void* pos_emb, int64_t P,
-                                     int64_t R, int64_t pe_stride_s, int64_t pe_stride_n, int pe_dtype, int64_t q_cutoff,
-                                     int64_t k_cutoff, int layer_norm, float eps, int dtype, void* stream) {
+extern "C" int rgd_rope_cache_append(const rgd_cache_append_args* args, void* stream) {
     const char* name = "rgd_rope_cache_append";
+    RGD_REQUIRE(args, RGD_ERR_INVALID, "%s: null arguments", name);
+    const auto& [B, T, Hq, Hkv, D, q, k, v, qo, k_cache, v_cache, num_pages, page_size, page_table, max_pages, table_stride,
+                 cache_lens, new_lens, pos_emb, P, R, pe_stride_s, pe_stride_n, q_cutoff, k_cutoff, pe_dtype, layer_norm, dtype,
+                 eps] = *args;
     rgd_ensure_init();
     RGD_REQUIRE(dtype == RGD_F16 || dtype == RGD_BF16, RGD_ERR_INVALID, "%s: Only support fp16 and bf16", name);
     RGD_REQUIRE(B >= 0 && T >= 0 && Hq >= 0 && Hkv >= 0 && num_pages >= 0 && max_pages >= 0, RGD_ERR_INVALID,
@@ -234,13 +232,13 @@ extern "C" int rgd_rope_cache_append(int64_t B, int64_t T, int64_t Hq, int64_t H
 
     AppendParams p;
     memset(&p, 0, sizeof(p));  // (heads 0: nothing to do for a tensor)
-    const rgd_tensor4* xs[3] = {q, k, v};
-    const rgd_tensor4* ys[3] = {qo, k_cache, v_cache};
+    const rgd_tensor4* xs[3] = {&q, &k, &v};
+    const rgd_tensor4* ys[3] = {&qo, &k_cache, &v_cache};
     for (int i = 0; i < 3; ++i) {
         AppendRows& a = p.t[i];
         const int64_t heads = i == 0 ? Hq : Hkv;
         if (heads == 0 || (i && num_pages == 0)) continue;
-        RGD_REQUIRE(xs[i] && xs[i]->ptr && ys[i] && ys[i]->ptr, RGD_ERR_INVALID, "%s: null tensor", name);
+        RGD_REQUIRE(xs[i]->ptr && ys[i]->ptr, RGD_ERR_INVALID, "%s: null tensor", name);
         a.x = xs[i]->ptr;
         a.y = ys[i]->ptr;
         a.sx[0] = xs[i]->stride_b, a.sx[1] = xs[i]->stride_h, a.sx[2] = xs[i]->stride_n;

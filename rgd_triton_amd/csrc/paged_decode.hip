@@ -47,13 +47,12 @@ size_t rgd_paged_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D)
     return (size_t)(plan + 2 * decode_grid(D) * (rows * 32 * chunks_of(D) + 32) * 4);
 }
 
-int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_tensor4* q, const rgd_tensor4* k_cache,
-                     const rgd_tensor4* v_cache, int64_t num_pages, int64_t page_size, const int32_t* page_table,
-                     int64_t max_pages, int64_t table_stride, const int32_t* seq_lens, const void* rel_weight, int64_t w_stride,
-                     int64_t num_buckets, int w_dtype, int64_t n_ranges, const int32_t* starts, const int32_t* buckets,
-                     const rgd_tensor4* o, float* lse, int dtype, float softmax_scale, void* workspace, size_t workspace_bytes,
-                     void* stream) {
+int rgd_paged_decode(const rgd_paged_decode_args* args, void* stream) {
     const char* name = "rgd_paged_decode";
+    RGD_REQUIRE(args, RGD_ERR_INVALID, "%s: null arguments", name);
+    const auto& [B, Hq, Hkv, D, q, k_cache, v_cache, o, num_pages, page_size, page_table, max_pages, table_stride, seq_lens,
+                 rel_weight, w_stride, num_buckets, n_ranges, starts, buckets, lse, workspace, workspace_bytes, w_dtype, dtype,
+                 softmax_scale] = *args;
     rgd_ensure_init();
     RGD_REQUIRE(dtype == RGD_F16 || dtype == RGD_BF16, RGD_ERR_INVALID, "%s: Only support fp16 and bf16", name);
     RGD_REQUIRE(B >= 0 && Hq >= 0 && Hkv >= 0 && num_pages >= 0 && max_pages >= 0, RGD_ERR_INVALID, "%s: negative shape", name);
@@ -66,9 +65,9 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
     if (B == 0 || Hq == 0) return RGD_OK;
     RGD_REQUIRE(Hkv >= 1 && Hq % Hkv == 0, RGD_ERR_INVALID, "%s: query heads must be a multiple of the key heads", name);
     const bool none = num_pages == 0 || max_pages == 0;  // no key can exist
-    RGD_REQUIRE(seq_lens && (none || (page_table && k_cache && k_cache->ptr && v_cache && v_cache->ptr)), RGD_ERR_INVALID,
+    RGD_REQUIRE(seq_lens && (none || (page_table && k_cache.ptr && v_cache.ptr)), RGD_ERR_INVALID,
                 "%s: null cache, page table or lengths", name);
-    RGD_REQUIRE(q && q->ptr && o && o->ptr, RGD_ERR_INVALID, "%s: null tensor", name);
+    RGD_REQUIRE(q.ptr && o.ptr, RGD_ERR_INVALID, "%s: null tensor", name);
     DecodeParams p;
     memset(&p, 0, sizeof(p));
     DecodeBias rel;
@@ -95,16 +94,16 @@ int rgd_paged_decode(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const rgd_te
         memcpy(rel.near, near, sizeof(near));
         bias = &rel;
     }
-    p.q = q->ptr;
-    p.o = o->ptr;
+    p.q = q.ptr;
+    p.o = o.ptr;
     p.lse = lse;
-    p.sq[0] = q->stride_b, p.sq[1] = q->stride_h;
-    p.so[0] = o->stride_b, p.so[1] = o->stride_h;
+    p.sq[0] = q.stride_b, p.sq[1] = q.stride_h;
+    p.so[0] = o.stride_b, p.so[1] = o.stride_h;
     if (!none) {
-        p.k = k_cache->ptr;
-        p.v = v_cache->ptr;
-        p.sk[0] = k_cache->stride_b, p.sk[1] = k_cache->stride_h, p.sk[2] = k_cache->stride_n;
-        p.sv[0] = v_cache->stride_b, p.sv[1] = v_cache->stride_h, p.sv[2] = v_cache->stride_n;
+        p.k = k_cache.ptr;
+        p.v = v_cache.ptr;
+        p.sk[0] = k_cache.stride_b, p.sk[1] = k_cache.stride_h, p.sk[2] = k_cache.stride_n;
+        p.sv[0] = v_cache.stride_b, p.sv[1] = v_cache.stride_h, p.sv[2] = v_cache.stride_n;
     }
     p.page_table = page_table;
     p.seq_lens = seq_lens;

@@ -720,6 +720,7 @@ class _RelativeRanges:
         self.starts, self.buckets, self.n, self.most = starts, buckets, len(starts), max(buckets)
         self.c_starts = (ctypes.c_int32 * self.n)(*starts)
         self.c_buckets = (ctypes.c_int32 * self.n)(*buckets)
+        self.starts_at, self.buckets_at = ctypes.addressof(self.c_starts), ctypes.addressof(self.c_buckets)
 
 
 @functools.lru_cache(maxsize=64, typed=True)
@@ -760,7 +761,7 @@ def relative_ranges(num_buckets, max_distance, bidirectional):
 
 
 # The functions below are called once per token, or between short kernels, where their host time is what a user waits for: tensor
-# attributes are read once, descriptors are packed bytes, the stream is asked for as a number.
+# attributes are read once, arguments are packed bytes, the stream is asked for as a number.
 _current_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _desc4 = _hip.desc4
@@ -926,31 +927,40 @@ def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_tabl
             return rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens, seq_cutoff,
                                         heads_second, norm_eps)
     if pos_emb is None:
-        pe = (None, 0, 0, 0, 0, _hip.RGD_F32)
+        table, P, R, ss, sn, table_code = 0, 0, 0, 0, 0, _hip.RGD_F32
     else:
         _, P, R = pos_emb.shape
         ss, sn, _ = pos_emb.stride()
-        pe = (pos_emb.data_ptr(), P, R, ss, sn, _hip.dtype_code(pos_emb.dtype))
+        table, table_code = pos_emb.data_ptr(), _hip.dtype_code(pos_emb.dtype)
     cq, ck = _cutoffs(seq_cutoff, 2**31 - 1, 2**31 - 1)
     qo = torch.empty_like(query)
-    sq, sk, sv, so, ck_s, cv_s = query.stride(), key.stride(), value.stride(), qo.stride(), k_cache.stride(), v_cache.stride()
-    rc = _hip.lib().rgd_rope_cache_append(
-        shape[0], shape[tok], shape[head], kshape[head], shape[3],
-        _desc4(query.data_ptr(), sq[0], sq[head], sq[tok]), _desc4(key.data_ptr(), sk[0], sk[head], sk[tok]),
-        _desc4(value.data_ptr(), sv[0], sv[head], sv[tok]), _desc4(qo.data_ptr(), so[0], so[head], so[tok]),
-        _desc4(k_cache.data_ptr(), ck_s[0], ck_s[2], ck_s[1]), _desc4(v_cache.data_ptr(), cv_s[0], cv_s[2], cv_s[1]),
-        cshape[0], cshape[1], page_table.data_ptr(), page_table.shape[1], page_table.stride(0), cache_lens.data_ptr(),
-        None if new_lens is None else new_lens.data_ptr(), *pe, cq, ck, norm_eps is not None, norm_eps or 0.0,
-        _hip.dtype_code(dtype), _raw_stream(index))
+    sq, sk, sv, so = query.stride(), key.stride(), value.stride(), qo.stride()
+    kcp, kcs, kch, _ = k_cache.stride()
+    vcp, vcs, vch, _ = v_cache.stride()
+    args = _hip.append_args(
+        shape[0], shape[tok], shape[head], kshape[head], shape[3], query.data_ptr(), sq[0], sq[head], sq[tok], key.data_ptr(), sk[0], sk[head], sk[tok],
+        value.data_ptr(), sv[0], sv[head], sv[tok], qo.data_ptr(), so[0], so[head], so[tok], k_cache.data_ptr(), kcp, kch, kcs, v_cache.data_ptr(), vcp,
+        vch, vcs, cshape[0], cshape[1], page_table.data_ptr(), page_table.shape[1], page_table.stride(0), cache_lens.data_ptr(),
+        0 if new_lens is None else new_lens.data_ptr(), table, P, R, ss, sn, cq, ck, table_code, norm_eps is not None,
+        _hip.dtype_code(dtype), norm_eps or 0.0)
+    rc = _hip.lib().rgd_rope_cache_append(args, _raw_stream(index))
     if rc:
         _hip.check(rc, "rgd_rope_cache_append")
-    for cache in (k_cache, v_cache):
-        if not cache.is_inference():  # (those have no version)
-            torch.autograd.graph.increment_version(cache)
+    if k_cache.is_inference() or v_cache.is_inference():  # (tensors made in inference mode have no version)
+        for cache in (k_cache, v_cache):
+            if not cache.is_inference():
+                torch.autograd.graph.increment_version(cache)
+    else:
+        torch.autograd.graph.increment_version((k_cache, v_cache))
     return qo
 
 
-_NO_BIAS = (None, 0, 0, _hip.RGD_F32, 0, None, None)
+_NO_BIAS = (0, 0, 0, 0, 0, 0)
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_workspace(B, Hq, Hkv, D):
+    return _hip.lib().rgd_paged_decode_workspace(B, Hq, Hkv, D)
 
 
 def paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight=None, max_distance=128, bidirectional=True,
@@ -986,22 +996,23 @@ def paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight
             return paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight, max_distance, bidirectional,
                                           softmax_scale, return_lse)
     B, _, Hq, D = shape
-    rel = _NO_BIAS
+    rel, rel_code = _NO_BIAS, _hip.RGD_F32
     if rel_weight is not None:
         r = relative_ranges(rel_weight.shape[0], max_distance, bool(bidirectional))
-        rel = (rel_weight.data_ptr(), rel_weight.stride(0), rel_weight.shape[0], _hip.dtype_code(rel_weight.dtype), r.n, r.c_starts,
-               r.c_buckets)
+        rel = (rel_weight.data_ptr(), rel_weight.stride(0), rel_weight.shape[0], r.n, r.starts_at, r.buckets_at)
+        rel_code = _hip.dtype_code(rel_weight.dtype)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
-    lib = _hip.lib()
-    nbytes = lib.rgd_paged_decode_workspace(B, Hq, cache[2], D)
+    nbytes = _decode_workspace(B, Hq, cache[2], D)
     ws = _hip.workspace(q.device, nbytes)
-    ck_s, cv_s = k_cache.stride(), v_cache.stride()
-    rc = lib.rgd_paged_decode(
-        B, Hq, cache[2], D, _desc4(q.data_ptr(), sq[0], sq[2], sq[1]), _desc4(k_cache.data_ptr(), ck_s[0], ck_s[2], ck_s[1]),
-        _desc4(v_cache.data_ptr(), cv_s[0], cv_s[2], cv_s[1]), cache[0], cache[1], page_table.data_ptr(), page_table.shape[1],
-        page_table.stride(0), seq_lens.data_ptr(), *rel, _desc4(o.data_ptr(), Hq * D, D, 0), None if lse is None else lse.data_ptr(),
-        _hip.dtype_code(dtype), 1.0 / math.sqrt(D) if softmax_scale is None else softmax_scale, ws.data_ptr(), nbytes, _raw_stream(index))
+    kcp, kcs, kch, _ = k_cache.stride()
+    vcp, vcs, vch, _ = v_cache.stride()
+    args = _hip.decode_args(
+        B, Hq, cache[2], D, q.data_ptr(), sq[0], sq[2], sq[1], k_cache.data_ptr(), kcp, kch, kcs, v_cache.data_ptr(), vcp, vch, vcs,
+        o.data_ptr(), Hq * D, D, 0, cache[0], cache[1], page_table.data_ptr(), page_table.shape[1], page_table.stride(0),
+        seq_lens.data_ptr(), *rel, 0 if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes, rel_code, _hip.dtype_code(dtype),
+        1.0 / math.sqrt(D) if softmax_scale is None else softmax_scale)
+    rc = _hip.lib().rgd_paged_decode(args, _raw_stream(index))
     if rc:
         _hip.check(rc, "rgd_paged_decode")
     return (o, lse) if return_lse else o

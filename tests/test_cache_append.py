@@ -132,12 +132,13 @@ def test_append_in_place_query_and_version():
         case = (2, 3, 3, 4, D, R, 16, BF, FP, True, False, True)
         s = {n: (None if t is None else t.cuda()) for n, t in _inputs(case, 260).items()}
         want = rope_cache_append_fn(s["q"], s["k"], s["v"], s["table"], s["k_cache"], s["v_cache"], s["pages"], s["lens"], norm_eps=1e-6)
-        d4 = lambda t, h, n: _hip.desc4(t.data_ptr(), t.stride(0), t.stride(h), t.stride(n))  # noqa: E731
-        rc = _hip.lib().rgd_rope_cache_append(
-            2, 3, 3, 4, D, d4(s["q"], 1, 2), d4(s["k"], 1, 2), d4(s["v"], 1, 2), d4(s["q"], 1, 2), d4(s["k_cache"], 2, 1), d4(s["v_cache"], 2, 1),
-            s["k_cache"].shape[0], 16, s["pages"].data_ptr(), s["pages"].shape[1], s["pages"].stride(0), s["lens"].data_ptr(), None,
-            s["table"].data_ptr(), s["table"].shape[1], R, s["table"].stride(0), s["table"].stride(1), 0, 2**31 - 1, 2**31 - 1, 1, 1e-6, 2,
-            _hip.stream_ptr(s["q"].device))
+        d4 = lambda t, h, n: (t.data_ptr(), t.stride(0), t.stride(h), t.stride(n))  # noqa: E731
+        args = _hip.append_args(
+            2, 3, 3, 4, D, *d4(s["q"], 1, 2), *d4(s["k"], 1, 2), *d4(s["v"], 1, 2), *d4(s["q"], 1, 2), *d4(s["k_cache"], 2, 1),
+            *d4(s["v_cache"], 2, 1), s["k_cache"].shape[0], 16, s["pages"].data_ptr(), s["pages"].shape[1], s["pages"].stride(0),
+            s["lens"].data_ptr(), 0, s["table"].data_ptr(), s["table"].shape[1], R, s["table"].stride(0), s["table"].stride(1), 2**31 - 1,
+            2**31 - 1, 0, 1, 2, 1e-6)
+        rc = _hip.lib().rgd_rope_cache_append(args, _hip.stream_ptr(s["q"].device))
         assert rc == 0 and torch.equal(s["q"], want)
     case = (2, 3, 4, 4, 64, 64, 16, BF, FP, False, False, True)
     s = {n: (None if t is None else t.cuda()) for n, t in _inputs(case, 260).items()}

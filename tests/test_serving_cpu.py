@@ -13,6 +13,7 @@ from serving_helpers import gen, randn, rotary, serving_oracle
 from rgd_triton_amd import _hip
 
 T4 = _hip.desc4(0x1000, 4096, 64, 64)
+D4 = (0x1000, 4096, 64, 64)
 BUF = ctypes.c_void_p(0x1000)
 
 
@@ -83,18 +84,28 @@ def test_oracle_bias_gradient_against_differences():
 # ------------------------------------------------------------------ refusals
 
 
+def _packed(pack, a):
+    """an argument structure from its members in order: descriptors as tuples, None for a null pointer or descriptor"""
+    flat = []
+    for name, x in a.items():
+        if x is None:
+            x = (0, 0, 0, 0) if name in ("q", "k", "v", "qo", "kc", "vc", "o") else 0
+        flat += x if isinstance(x, tuple) else (x,)
+    return pack(*flat)
+
+
 def _append(**kw):
-    a = dict(B=1, T=2, Hq=4, Hkv=2, D=64, q=T4, k=T4, v=T4, qo=T4, kc=T4, vc=T4, pages=8, size=16, table=BUF, per=4, stride=4, lens=BUF,
-             new=None, pe=BUF, P=64, R=64, ss=4096, sn=64, pdt=0, cq=99, ck=99, ln=0, eps=0.0, dt=2)
+    a = dict(B=1, T=2, Hq=4, Hkv=2, D=64, q=D4, k=D4, v=D4, qo=D4, kc=D4, vc=D4, pages=8, size=16, table=0x1000, per=4, stride=4,
+             lens=0x1000, new=None, pe=0x1000, P=64, R=64, ss=4096, sn=64, cq=99, ck=99, pdt=0, ln=0, dt=2, eps=0.0)
     a.update(kw)
-    return _hip.lib().rgd_rope_cache_append(*a.values(), None)
+    return _hip.lib().rgd_rope_cache_append(_packed(_hip.append_args, a), None)
 
 
 def _decode(**kw):
-    a = dict(B=1, Hq=4, Hkv=2, D=64, q=T4, kc=T4, vc=T4, pages=8, size=16, table=BUF, per=4, stride=4, lens=BUF, w=None, ws=0, nb=0, wdt=0,
-             n=0, starts=None, buckets=None, o=T4, lse=None, dt=2, scale=0.125, work=BUF, bytes=1 << 30)
+    a = dict(B=1, Hq=4, Hkv=2, D=64, q=D4, kc=D4, vc=D4, o=D4, pages=8, size=16, table=0x1000, per=4, stride=4, lens=0x1000, w=None, ws=0,
+             nb=0, n=0, starts=None, buckets=None, lse=None, work=0x1000, bytes=1 << 30, wdt=0, dt=2, scale=0.125)
     a.update(kw)
-    return _hip.lib().rgd_paged_decode(*a.values(), None)
+    return _hip.lib().rgd_paged_decode(_packed(_hip.decode_args, a), None)
 
 
 def test_append_refusals():
@@ -114,6 +125,7 @@ def test_append_refusals():
     assert _append(size=1 << 20, per=1 << 12) == -2 and b"2^31" in err()
     assert _append(B=1 << 20, T=1 << 12) == -2
     assert _append(B=1 << 14, T=1 << 14, Hq=2, Hkv=1) == -2 and b"one launch" in err()
+    assert _hip.lib().rgd_rope_cache_append(None, None) == -1 and b"null arguments" in err()
     # nothing to do is no error
     assert _append(T=0) == 0 and _append(B=0) == 0 and _append(Hq=0, Hkv=0) == 0
 
@@ -130,14 +142,16 @@ def test_decode_refusals():
     assert _decode(q=None) == -1 and _decode(o=None) == -1
     assert _decode(size=1 << 20, per=1 << 12) == -2
     assert _decode(B=1 << 22, Hq=4) == -2 and b"query rows" in err()
-    starts, buckets = (ctypes.c_int32 * 3)(-5, 0, 3), (ctypes.c_int32 * 3)(0, 1, 2)
-    rel = dict(w=BUF, ws=4, nb=3, n=3, starts=starts, buckets=buckets)
+    up, down, ids = (ctypes.c_int32 * 3)(-5, 0, 3), (ctypes.c_int32 * 3)(-5, 3, 0), (ctypes.c_int32 * 3)(0, 1, 2)
+    starts, buckets = ctypes.addressof(up), ctypes.addressof(ids)
+    rel = dict(w=0x1000, ws=4, nb=3, n=3, starts=starts, buckets=buckets)
     assert _decode(**{**rel, "wdt": 7}) == -1 and b"bias weights" in err()
     assert _decode(**{**rel, "nb": 2}) == -1 and b"bucket outside" in err()
     assert _decode(**{**rel, "n": 0}) == -1 and _decode(**{**rel, "n": 257}) == -1 and _decode(**{**rel, "starts": None}) == -1
-    assert _decode(**{**rel, "starts": (ctypes.c_int32 * 3)(-5, 3, 0)}) == -1 and b"ascend" in err()
+    assert _decode(**{**rel, "starts": ctypes.addressof(down)}) == -1 and b"ascend" in err()
     need = _hip.lib().rgd_paged_decode_workspace(1, 4, 2, 64)
     assert need > 0 and _decode(bytes=need - 1) == -4 and b"workspace" in err() and _decode(work=None) == -4
+    assert _hip.lib().rgd_paged_decode(None, None) == -1 and b"null arguments" in err()
     assert _decode(B=0) == 0 and _decode(Hq=0, Hkv=1) == 0
 
 
