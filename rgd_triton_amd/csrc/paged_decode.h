@@ -5,7 +5,7 @@
 // Bound by memory: every cached key and value is read once, 4 D bytes per token and key head, for 4 D group operations.
 //
 // Work.  A unit is (sequence, key head, 16 of the key head's query heads); its keys are cut into tiles of 32.  The tiles of all
-// units, in one row, are dealt to the wavefronts in equal runs: every wavefront finds its run from the lengths on the GPU, so
+// units (of one key head per bundle, see below), in one row, are dealt to the wavefronts in equal runs: every wavefront finds its run from the lengths on the GPU, so
 // the host need not know them, one long sequence fills the chip like many short ones, and a ragged batch leaves no wavefront
 // with more than a tile over the others.  A run that holds a whole unit writes its output; pieces of a unit that several
 // wavefronts share leave partial results in the workspace (at most two per wavefront: one unit begun earlier, one not ended),
@@ -27,7 +27,7 @@
 //
 // Measured (this launch / the merge; a read that streams 512 MB reaches 6.6 TB/s): one sequence of 131000 keys, 32 / 8 heads,
 // D = 128: 86 / 7 us, 6.2 TB/s; 64 sequences to 4100 keys, the same heads: 106 / 5 us, 5.5 TB/s; 19 to 2000 keys, 24 heads,
-// D = 80, bias, pages of 5: 45 / 5 us; one of 200 keys, 16 heads, D = 64: 5.3 / 3.6 us.  What a launch takes beyond its
+// D = 80, bias, pages of 5: 40 / 5 us; one of 200 keys, 16 heads, D = 64: 5.3 / 3.6 us.  What a launch takes beyond its
 // bytes, about 15 us, is the chain of loads in front of the first step (lengths, page numbers, keys), the last steps, in which
 // the wavefronts run out one by one, and the merge.
 #pragma once
@@ -51,7 +51,9 @@ struct DecodeParams {
     const int32_t* seq_lens;
     int64_t table_stride;
     int32_t capacity;  // positions of a page table row
-    int B, Hq, group, head_tiles, units;  // units = key heads * head_tiles, per sequence
+    int B, Hq, group, head_tiles;
+    int units;         // of a sequence: key heads / heads of a bundle * head_tiles
+    int bundle_log;    // 2^bundle_log key heads in a bundle
     int D, num_pages;
     FastDiv div_page;
     float scale;
@@ -115,19 +117,20 @@ constexpr float DEC_LAZY = 5.5f;
 // What is left is at most (2^-7 + 2^-8) p, its own rounding 2^-14.4 p.
 constexpr float DEC_HIGH = 1.0f - 1.0f / 128;
 
-// NC: 32-channel chunks of the head dim (DP = 32 NC).  SMALL: D < 8, rows are read element by element.
+// NC: 32-channel chunks of the head dim (DP = 32 NC).  SMALL: D < 8, rows are read element by element.  LINES: D = DP is 64 or 128,
+// rows of token-major heads are whole 128-byte lines, which no other wavefront reads: loads stream.
+// Else lines are shared by neighbouring heads: loads do not stream, and the key heads that fill lines together are a bundle, whose
+// wavefronts take the same tiles of one head each, on one XCD, side by side: the first to come fetches the line for all of
+// them.  19 x 24 heads, lengths to 2000, streaming / not / not and in bundles: D = 16: 28 / 27 / 19 us, D = 32: 28 / 28 / 23, D = 40:
+// 37 / - / 30, D = 80: 48 / 45 / 40, D = 112: 59 / - / 53; one of 131000 keys, 8 key heads, D = 80: 94 / 82 / 76, D = 128 (no bundles):
+// 95 / 104.
 // The lanes look up the 32 keys' pages together and pass the row addresses around (20 cross-lane moves a step), whatever the
 // page size: a variant for pages of whole groups of 8 keys, in which a lane needs two page numbers and no moves, was no faster
 // ((19 x 24 heads, D = 128, lengths to 2000) pages of 16: 54.4 us this way, 54.1 that).
-template <typename T, int NC, bool SMALL, bool BIAS>
+template <typename T, int NC, bool SMALL, bool LINES, bool BIAS>
 __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams p,
                                                           const std::conditional_t<BIAS, DecodeBias, DecodeNoBias> rel) {
     constexpr int DP = 32 * NC, VE = DP / 16, VW = VE / 2;
-    // Where rows of token-major heads fill whole 128-byte lines (D = 64, 128) no other wavefront reads a line: loads stream.  Else
-    // neighbouring heads share lines and they do not; and where a line holds whole rows of several heads, neighbouring runs go
-    // to one XCD, whose L2 then has them.  Streaming / not / not and by XCD: (19 x 24 heads, lengths to 2000) D = 16: 28 / 27 /
-    // 20 us, D = 32: 28 / 28 / 24, D = 80: 47 / 44 / 44; one of 131000 keys, 8 key heads, D = 80: 94 / 82 / 88, D = 128: 95 / 104 / 111.
-    constexpr bool ALONE = NC % 2 == 0, BY_XCD = NC == 1;
     // BIAS, by the number of ranges (for 256 of them 8 wavefronts fit a compute unit, for 32 all 12 of the small head dims do:
     // D = 64, 24 heads, 19 lengths to 2000 with bias 37 us instead of 42)
     static_assert(DEC_NEAR == 4 * 64, "a dword per lane");
@@ -135,10 +138,13 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
     int *s_start = nullptr, *s_bucket = nullptr;
     float (*s_w)[16] = nullptr;
 
-    const int wave = BY_XCD && gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
+    // run: the wavefront's part of the row of tiles; sub: its key head of a bundle
+    const int bl = p.bundle_log, bundle = 1 << bl, runs = gridDim.x >> bl;
+    const int sub = blockIdx.x >> 3 & (bundle - 1);
+    const int run = (blockIdx.x >> (3 + bl) << 3) + (blockIdx.x & 7);  // (workgroups go round the 8 XCDs)
     const int lane = threadIdx.x;
     const int n16 = lane & 15, g = lane >> 4;
-    const int D = p.D;
+    const int D = LINES ? DP : p.D;
     auto length = [&](int b) {
         const int n = p.seq_lens[b];
         return n < 0 ? 0 : (n < p.capacity ? n : p.capacity);
@@ -173,9 +179,9 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
     int64_t total = last_of(incl);
     for (int b0 = 64; b0 < p.B; b0 += 64) total += last_of(scan(b0 + lane < p.B ? tiles_of(length(b0 + lane)) : 0));
     total *= p.units;
-    const int64_t even = total <= INT32_MAX ? (int64_t)((uint32_t)total / gridDim.x) : total / gridDim.x, rest = total - even * gridDim.x;
-    int64_t x = even * wave + min((int64_t)wave, rest);
-    const int64_t x_end = x + even + (wave < rest ? 1 : 0);
+    const int64_t even = total <= INT32_MAX ? (int64_t)((uint32_t)total / (uint32_t)runs) : total / runs, rest = total - even * runs;
+    int64_t x = even * run + min((int64_t)run, rest);
+    const int64_t x_end = x + even + (run < rest ? 1 : 0);
     if (x >= x_end) return;
     int b = 0;
     int64_t base = 0;  // first tile of sequence b
@@ -195,7 +201,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
 
     // ---- a piece: tiles tile0 .. tile1 - 1 of one unit
     struct Piece {
-        int b, unit, len, ntiles, tile0, tile1, head0, heads;
+        int b, unit, len, ntiles, tile0, tile1, hk, head0, heads;
     };
     auto piece_at = [&]() {
         Piece c;
@@ -206,9 +212,10 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
         c.unit = in_seq <= INT32_MAX ? (int)((uint32_t)in_seq / (uint32_t)c.ntiles) : (int)(in_seq / c.ntiles);
         c.tile0 = (int)(in_seq - (int64_t)c.unit * c.ntiles);
         c.tile1 = (int)min((int64_t)c.ntiles, c.tile0 + (x_end - x));
-        const int hk = c.unit / p.head_tiles;
-        c.head0 = hk * p.group + (c.unit - hk * p.head_tiles) * 16;
-        c.heads = min(16, (hk + 1) * p.group - c.head0);
+        const int of = c.unit / p.head_tiles;
+        c.hk = (of << bl) + sub;
+        c.head0 = c.hk * p.group + (c.unit - of * p.head_tiles) * 16;
+        c.heads = min(16, (c.hk + 1) * p.group - c.head0);
         return c;
     };
 
@@ -234,9 +241,8 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
 
     auto aim = [&](const Piece& c) __attribute__((always_inline)) {
         load_len = c.len;
-        const int hk = c.unit / p.head_tiles;
-        kbase = static_cast<const T*>(p.k) + hk * p.sk[1];
-        vbase = static_cast<const T*>(p.v) + hk * p.sv[1];
+        kbase = static_cast<const T*>(p.k) + c.hk * p.sk[1];
+        vbase = static_cast<const T*>(p.v) + c.hk * p.sv[1];
         table = p.page_table + c.b * p.table_stride;
     };
     // (only the sequence's own page numbers are read; one without keys reads its first, and what that leads to is not used)
@@ -264,7 +270,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
                     kf[a][c] = r.v;
                 } else {
                     uint32_t r[4];
-                    load_dwords<4, ALONE>(reinterpret_cast<const char*>(row + kstart[c]), r);
+                    load_dwords<4, LINES>(reinterpret_cast<const char*>(row + kstart[c]), r);
                     kf[a][c] = u32x4{r[0], r[1], r[2], r[3]};
                 }
             }
@@ -278,7 +284,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
                 const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
                 vr[i][0] = r[min(vstart, D - 1)] | (uint32_t)r[min(vstart + 1, D - 1)] << 16;
             } else {
-                load_dwords<VW, ALONE>(reinterpret_cast<const char*>(row + vstart), vr[i]);
+                load_dwords<VW, LINES>(reinterpret_cast<const char*>(row + vstart), vr[i]);
             }
         }
     };
@@ -317,9 +323,9 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
         l += xor_lanes(l, 16);
         l += xor_lanes(l, 32);
         if (lane == 0) {
-            int* plan = &p.plan[2 * ((int64_t)cur.b * p.units + cur.unit)];
-            if (begins) plan[0] = wave;
-            if (ends) plan[1] = wave;
+            int* plan = &p.plan[2 * ((((int64_t)cur.b * p.units + cur.unit) << bl) + sub)];
+            if (begins) plan[0] = run;
+            if (ends) plan[1] = run;
         }
         if (n16 < heads) {
             if (begins && ends) {
@@ -341,7 +347,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
                 }
                 if (p.lse && g == 0) p.lse[(int64_t)cur.b * p.Hq + head0 + n16] = l == 0.f ? -INFINITY : (ref == -INFINITY ? 0.f : ref) + logf(l);
             } else {
-                float* slot = p.part + (int64_t)(2 * wave + (begins ? 1 : 0)) * ((int64_t)p.part_rows * DP + 32);
+                float* slot = p.part + (int64_t)(2 * ((run << bl) + sub) + (begins ? 1 : 0)) * ((int64_t)p.part_rows * DP + 32);
                 float out[4 * VE];
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
@@ -533,12 +539,12 @@ __global__ __launch_bounds__(THREADS) void paged_decode_merge_kernel(const Decod
     __shared__ float s_red[THREADS / 64];
     const int b = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
     const int hk = h / p.group, in_group = h - hk * p.group;
-    const int unit = hk * p.head_tiles + (in_group >> 4), row = in_group & 15;
-    const int* plan = &p.plan[2 * ((int64_t)b * p.units + unit)];
+    const int bl = p.bundle_log, sub = hk & ((1 << bl) - 1), unit = (hk >> bl) * p.head_tiles + (in_group >> 4), row = in_group & 15;
+    const int* plan = &p.plan[2 * ((((int64_t)b * p.units + unit) << bl) + sub)];
     struct { int x, y; } span = {plan[0], plan[1]};
     if (span.x == span.y) return;  // one piece: written already
     const int64_t slot_size = (int64_t)p.part_rows * DP + 32;
-    auto slot = [&](int w) { return p.part + (int64_t)(2 * w + (w == span.x ? 1 : 0)) * slot_size; };
+    auto slot = [&](int w) { return p.part + (int64_t)(2 * ((w << bl) + sub) + (w == span.x ? 1 : 0)) * slot_size; };
     const int tid = threadIdx.x, grp = tid >> 5, c4 = (tid & 31) * 4;
     auto over_all = [&](float v, auto op) {  // v over the workgroup, op(a, b)
         __syncthreads();

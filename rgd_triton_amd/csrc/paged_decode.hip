@@ -12,27 +12,29 @@ int chunks_of(int64_t D) { return (int)((D + 31) / 32); }
 // (D = 128, 24 heads, 19 lengths to 2000) 58 / 54 / 57 us.
 int64_t decode_grid(int64_t D) { return (int64_t)rgd_num_cus() * 4 * (D <= 64 ? 3 : 2); }
 
-template <typename T, int NC, bool SMALL>
+template <typename T, int NC, bool SMALL, bool LINES>
 int decode_launch(const DecodeParams& p, const DecodeBias* rel, unsigned grid, bool merge, hipStream_t s) {
     const size_t lds = rel ? DEC_NEAR + (rel->half ? 2 * rel->half : 1) * 2 * sizeof(int) + rel->n_ranges * 16 * sizeof(float) : 0;
-    const hipError_t e = rel ? rgd_launch(paged_decode_kernel<T, NC, SMALL, true>, dim3(grid), dim3(64), lds, s, p, *rel)
-                             : rgd_launch(paged_decode_kernel<T, NC, SMALL, false>, dim3(grid), dim3(64), 0, s, p, DecodeNoBias{});
+    const hipError_t e = rel ? rgd_launch(paged_decode_kernel<T, NC, SMALL, LINES, true>, dim3(grid), dim3(64), lds, s, p, *rel)
+                             : rgd_launch(paged_decode_kernel<T, NC, SMALL, LINES, false>, dim3(grid), dim3(64), 0, s, p, DecodeNoBias{});
     const int rc = rgd_launch_status("rgd_paged_decode", e);
     if (rc != RGD_OK || !merge) return rc;
     // pieces of a unit, if all units are alike: beyond what the small workgroup keeps in flight at once the large one is faster
     const dim3 heads((unsigned)p.B * (unsigned)p.Hq);
-    const bool many = grid / ((int64_t)p.B * p.units) > 64;
+    const bool many = grid / ((int64_t)p.B * p.units << p.bundle_log) > 64;
     return rgd_launch_status("rgd_paged_decode", many ? rgd_launch(paged_decode_merge_kernel<T, NC, SMALL, 1024>, heads, dim3(1024), 0, s, p)
                                                       : rgd_launch(paged_decode_merge_kernel<T, NC, SMALL, 256>, heads, dim3(256), 0, s, p));
 }
 
 template <typename T> int decode_dispatch(const DecodeParams& p, const DecodeBias* rel, unsigned grid, bool merge, hipStream_t s) {
-    if (p.D < 8) return decode_launch<T, 1, true>(p, rel, grid, merge, s);
+    if (p.D < 8) return decode_launch<T, 1, true, false>(p, rel, grid, merge, s);
+    if (p.D == 64) return decode_launch<T, 2, false, true>(p, rel, grid, merge, s);
+    if (p.D == 128) return decode_launch<T, 4, false, true>(p, rel, grid, merge, s);
     switch (chunks_of(p.D)) {
-        case 1: return decode_launch<T, 1, false>(p, rel, grid, merge, s);
-        case 2: return decode_launch<T, 2, false>(p, rel, grid, merge, s);
-        case 3: return decode_launch<T, 3, false>(p, rel, grid, merge, s);
-        default: return decode_launch<T, 4, false>(p, rel, grid, merge, s);
+        case 1: return decode_launch<T, 1, false, false>(p, rel, grid, merge, s);
+        case 2: return decode_launch<T, 2, false, false>(p, rel, grid, merge, s);
+        case 3: return decode_launch<T, 3, false, false>(p, rel, grid, merge, s);
+        default: return decode_launch<T, 4, false, false>(p, rel, grid, merge, s);
     }
 }
 
@@ -113,7 +115,6 @@ int rgd_paged_decode(const rgd_paged_decode_args* args, void* stream) {
     p.Hq = (int)Hq;
     p.group = (int)(Hq / Hkv);
     p.head_tiles = (p.group + 15) / 16;
-    p.units = (int)Hkv * p.head_tiles;
     p.part_rows = p.group < 16 ? p.group : 16;
     p.D = (int)D;
     p.num_pages = (int)num_pages;
@@ -123,7 +124,7 @@ int rgd_paged_decode(const rgd_paged_decode_args* args, void* stream) {
     RGD_REQUIRE(workspace && workspace_bytes >= rgd_paged_decode_workspace(B, Hq, Hkv, D), RGD_ERR_WORKSPACE,
                 "%s: workspace of %zu bytes, needs %zu", name, workspace_bytes, rgd_paged_decode_workspace(B, Hq, Hkv, D));
     p.plan = static_cast<int*>(workspace);
-    p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (B * p.units * 2 * (int64_t)sizeof(int) + 15) / 16 * 16);
+    p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (B * Hkv * p.head_tiles * 2 * (int64_t)sizeof(int) + 15) / 16 * 16);
     if (none) {
         const dim3 rows((unsigned)(B * Hq));
         return rgd_launch_status(name, dtype == RGD_F16 ? rgd_launch(paged_decode_empty_kernel<f16_t>, rows, dim3(64), 0, s, p)
@@ -131,8 +132,13 @@ int rgd_paged_decode(const rgd_paged_decode_args* args, void* stream) {
     }
     // more wavefronts than there can be tiles have nothing to do; units of one tile are in no two wavefronts
     const int64_t most = p.capacity > DEC_TILE ? (p.capacity + DEC_TILE - 1) / DEC_TILE : 1;
-    const int64_t tiles = B * p.units * most;
+    const int64_t tiles = B * Hkv * p.head_tiles * most;
     const unsigned grid = (unsigned)(tiles < decode_grid(D) ? tiles : decode_grid(D));
+    // bundles where rows of neighbouring key heads touch: the fewest heads that end on a line, at most 8 (odd head dims)
+    p.bundle_log = 0;
+    if (p.sk[1] == D && p.sv[1] == D)
+        while (p.bundle_log < 3 && (D * 2 << p.bundle_log) % 128 && Hkv % (2 << p.bundle_log) == 0 && grid % (16 << p.bundle_log) == 0) ++p.bundle_log;
+    p.units = (int)(Hkv >> p.bundle_log) * p.head_tiles;
     return dtype == RGD_F16 ? decode_dispatch<f16_t>(p, bias, grid, most > 1, s) : decode_dispatch<bf16_t>(p, bias, grid, most > 1, s);
 }
 

@@ -71,6 +71,27 @@ def test_decode_matches_definition(case):
     assert (o.cpu()[empty] == 0).all() and (lse.cpu()[empty] == -math.inf).all()
 
 
+LENGTHS = [0, 1, 31, 32, 33, 64, 65, 100, 127, 128, 129, 200, 255, 256, 300, 330]
+BUNDLES = [  # 2, 4 and 8 key heads whose rows end on a 128-byte line together, and fewer where the head count ends earlier
+    (40, 2, 32, 16, LENGTHS, BF, 8),
+    (4, 4, 16, 4, LENGTHS * 2, HF, 0),
+    (8, 8, 80, 16, LENGTHS, HF, 32),
+    (8, 8, 112, 48, LENGTHS, BF, 0),
+    (16, 8, 59, 8, LENGTHS, BF, 0),
+    (8, 8, 40, 5, LENGTHS, HF, 16),
+    (12, 12, 80, 16, LENGTHS, BF, 0),
+    (6, 6, 5, 16, LENGTHS, BF, 0),
+    (8, 8, 40, 16, [4000, 1, 3999, 0, 2500, 3000, 4000, 3500], BF, 16),
+]
+
+
+@pytest.mark.parametrize("case", BUNDLES)
+def test_decode_heads_that_share_lines(case):
+    s = _inputs(case, 370 + BUNDLES.index(case))
+    o, lse = _run(s)
+    check_decode(o, lse, _ref(s), max(case[4]), case[2])
+
+
 @pytest.mark.parametrize("both", [False, True])
 @pytest.mark.parametrize("nb,md,wdtype", [(32, 128, FP), (64, 600, BF), (8, 5, HF), (256, 300, FP)])
 def test_decode_relative_bias(nb, md, wdtype, both):
