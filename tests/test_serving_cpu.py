@@ -4,6 +4,8 @@ import bisect
 import ctypes
 import inspect
 import math
+import re
+import struct
 
 import pytest
 import torch
@@ -106,6 +108,21 @@ def _decode(**kw):
              nb=0, n=0, starts=None, buckets=None, lse=None, work=0x1000, bytes=1 << 30, wdt=0, dt=2, scale=0.125)
     a.update(kw)
     return _hip.lib().rgd_paged_decode(_packed(_hip.decode_args, a), None)
+
+
+@pytest.mark.parametrize("name,pack", [("rgd_cache_append_args", _hip.append_args), ("rgd_paged_decode_args", _hip.decode_args)])
+def test_argument_structures_are_the_headers(name, pack):
+    """the packed bytes have the members of the header's structure, in its order"""
+    text = re.sub(r"/\*.*?\*/", "", open(_hip.HEADER_PATH).read(), flags=re.S)
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S).group(1)
+    kinds = {"int64_t": "q", "int32_t": "i", "float": "f", "size_t": "N", "rgd_tensor4": "Pqqq"}
+    want = ""
+    for line in filter(None, (x.strip() for x in body.split(";"))):
+        kind, names = re.match(r"((?:const )?\w+ ?\*?) ?(.*)", line, flags=re.S).groups()
+        want += ("P" if "*" in line else kinds[kind.strip()]) * len(names.split(","))
+    fmt = re.sub(r"(\d+)([a-zA-Z])", lambda m: m.group(2) * int(m.group(1)), pack.__self__.format.lstrip("@"))
+    assert fmt.rstrip("x") == want
+    assert len(fmt) - len(want) == -struct.calcsize("@" + want) % 8  # padded to the structure's alignment
 
 
 def test_append_refusals():
