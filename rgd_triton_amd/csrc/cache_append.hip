@@ -91,12 +91,15 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const AppendParams p)
     const uint32_t head0 = (a.token_inner ? outer : inner) * U;
     const uint32_t tok = a.token_inner ? inner : outer;
 
-    const T* from = static_cast<const T*>(a.x) + b * a.sx[0] + tok * a.sx[2];
+    // (padding is not read, q's reads the sequence's first row: 8 prompts half of padding 133 -> 110 us, without new_lens 141.5 -> 142.4)
+    bool live = !p.new_lens || static_cast<int>(tok) < p.new_lens[b];
+    if (!live && which != 0) return;
+    const T* from = static_cast<const T*>(a.x) + b * a.sx[0] + (live ? tok : 0u) * a.sx[2];
     T raw[U][VEC];
 #pragma unroll
     for (int u = 0; u < U; ++u) load_row<T, VEC, WIDE>(from + min(head0 + u, a.heads - 1) * a.sx[1], first, D, raw[u]);
     const int64_t pos = static_cast<int64_t>(p.cache_lens[b]) + tok;
-    const bool live = pos >= 0 && pos < p.capacity && (!p.new_lens || static_cast<int>(tok) < p.new_lens[b]);
+    live = live && pos >= 0 && pos < p.capacity;
     T* y = static_cast<T*>(a.y);
     const bool turn = which != 2 && live && first < p.R && pos < a.cutoff;
     float sin[VEC], cos[VEC];
