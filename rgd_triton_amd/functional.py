@@ -767,6 +767,13 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _desc4 = _hip.desc4
 
 
+@functools.lru_cache(maxsize=256)
+def _bias_workspaces(nheads, seqlen_q, seqlen_k, num_buckets, code):
+    lib = _hip.lib()
+    return (lib.rgd_rel_bias_fwd_workspace(nheads, seqlen_q, seqlen_k, code),
+            lib.rgd_rel_bias_bwd_workspace(nheads, seqlen_q, seqlen_k, num_buckets))
+
+
 def _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, kernel_cache):
     wstride = weight.stride()
     device = weight.device
@@ -782,7 +789,7 @@ def _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, kernel_c
     num_buckets, nheads = weight.shape
     bias = torch.empty((1, nheads, seqlen_q, seqlen_k), dtype=dtype, device=device)
     lib, code = _hip.lib(), _hip.dtype_code(dtype)
-    nbytes = lib.rgd_rel_bias_fwd_workspace(nheads, seqlen_q, seqlen_k, code)  # 0 for all but large matrices
+    nbytes = _bias_workspaces(nheads, seqlen_q, seqlen_k, num_buckets, code)[0]  # 0 for all but large matrices
     ws = _hip.workspace(device, nbytes) if nbytes else None
     rc = lib.rgd_rel_bias_fwd(nheads, seqlen_q, seqlen_k, weight.data_ptr(), wstride[0], num_buckets, _hip.dtype_code(weight.dtype),
                               ranges.n, ranges.c_starts, ranges.c_buckets, q_offset,
@@ -805,10 +812,11 @@ def _relative_bias_grad(dbias, num_buckets, nheads, seqlen_q, seqlen_k, ranges, 
             return _relative_bias_grad(dbias, num_buckets, nheads, seqlen_q, seqlen_k, ranges, q_offset, wdtype)
     dw = torch.empty((num_buckets, nheads), dtype=wdtype, device=device)
     lib = _hip.lib()
-    nbytes = lib.rgd_rel_bias_bwd_workspace(nheads, seqlen_q, seqlen_k, num_buckets)
+    code = _hip.dtype_code(dbias.dtype)
+    nbytes = _bias_workspaces(nheads, seqlen_q, seqlen_k, num_buckets, code)[1]
     ws = _hip.workspace(device, nbytes)
     rc = lib.rgd_rel_bias_bwd(nheads, seqlen_q, seqlen_k, _desc4(dbias.data_ptr(), 0, stride[1], stride[2]),
-                              _hip.dtype_code(dbias.dtype), ranges.n, ranges.c_starts, ranges.c_buckets, q_offset, dw.data_ptr(),
+                              code, ranges.n, ranges.c_starts, ranges.c_buckets, q_offset, dw.data_ptr(),
                               nheads, num_buckets, _hip.dtype_code(wdtype), ws.data_ptr(), nbytes, _raw_stream(index))
     if rc:
         _hip.check(rc, "rgd_rel_bias_bwd")
@@ -817,18 +825,28 @@ def _relative_bias_grad(dbias, num_buckets, nheads, seqlen_q, seqlen_k, ranges, 
 
 class Relative_Bias_Func(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, kernel_cache):
-        ctx.args = (weight.shape[0], weight.shape[1], seqlen_q, seqlen_k, ranges, q_offset, weight.dtype)
-        ctx.kernel_cache = kernel_cache
-        return _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, kernel_cache)
+    def forward(ctx, weight, call):
+        ctx.weight, ctx.call = (*weight.shape, weight.dtype), call
+        return _relative_bias(weight, *call)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dbias):
-        _no_capture("Relative_Bias_Func.backward")
-        if ctx.kernel_cache is not None:
-            _seen(ctx.kernel_cache, "bwd", _sig(dbias))
-        return _relative_bias_grad(dbias, *ctx.args), None, None, None, None, None, None
+        # (once_differentiable costs 5 us, so only what could be differentiated again passes through it)
+        if torch.is_grad_enabled() and dbias.requires_grad:
+            return _relative_bias_once(ctx, dbias)
+        return _relative_bias_backward(ctx, dbias)
+
+
+def _relative_bias_backward(ctx, dbias):
+    _no_capture("Relative_Bias_Func.backward")
+    num_buckets, nheads, wdtype = ctx.weight
+    seqlen_q, seqlen_k, ranges, q_offset, _, kernel_cache = ctx.call
+    if kernel_cache is not None:
+        _seen(kernel_cache, "bwd", _sig(dbias))
+    return _relative_bias_grad(dbias, num_buckets, nheads, seqlen_q, seqlen_k, ranges, q_offset, wdtype), None
+
+
+_relative_bias_once = torch.autograd.function.once_differentiable(_relative_bias_backward)
 
 
 def relative_position_bias_fn(weight, seqlen_q, seqlen_k, max_distance=128, bidirectional=True, q_offset=0, dtype=None,
@@ -841,7 +859,7 @@ def relative_position_bias_fn(weight, seqlen_q, seqlen_k, max_distance=128, bidi
         weight = weight.contiguous()
     ranges = relative_ranges(weight.shape[0], max_distance, bool(bidirectional))
     if torch.is_grad_enabled() and weight.requires_grad:
-        return Relative_Bias_Func.apply(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype or weight.dtype, kernel_cache)
+        return Relative_Bias_Func.apply(weight, (seqlen_q, seqlen_k, ranges, q_offset, dtype or weight.dtype, kernel_cache))
     return _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype or weight.dtype, kernel_cache)
 
 
