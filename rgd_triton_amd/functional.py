@@ -42,17 +42,22 @@ def _lastdim_contig(*ts):
 
 
 def _seen(cache, field, key):
-    """True if this call signature already went through validation with this cache object."""
+    """True if a call with this signature has passed every check with this cache object."""
     if cache is None:
         return False
+    plans = getattr(cache, field, None)
+    return plans is not None and key in plans
+
+
+def _remember(cache, field, key):
+    """Keeps the signature of a call that has passed every check: a refused one has to be refused again."""
+    if cache is None:
+        return
     plans = getattr(cache, field, None)
     if plans is None:
         plans = set()
         setattr(cache, field, plans)
-    if key in plans:
-        return True
     plans.add(key)
-    return False
 
 
 def _no_capture(what):
@@ -104,9 +109,11 @@ class RMS_Func(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, norm_eps=1e-6, kernel_cache=None):
         x, w = _lastdim_contig(x, w)
-        if not _seen(kernel_cache, "fwd", _sig(x, w)):
+        key = _sig(x, w)
+        if not _seen(kernel_cache, "fwd", key):
             _check_rows(x)
             assert w.is_cuda and w.dtype in _FLOATS, "Only support fp16, bf16, and fp32"
+            _remember(kernel_cache, "fwd", key)
         shared, w_sb = _w_layout(w, x)
         B, T, C = x.shape
         y = torch.empty_like(x)
@@ -126,8 +133,8 @@ class RMS_Func(torch.autograd.Function):
         x, w = ctx.saved_tensors
         shared, w_sb = ctx.w_layout
         B, T, C = x.shape
-        _seen(ctx.kernel_cache, "bwd", _sig(x, w, dy))
-        _seen(ctx.kernel_cache, "bwd_dw", _sig(w))
+        _remember(ctx.kernel_cache, "bwd", _sig(x, w, dy))
+        _remember(ctx.kernel_cache, "bwd_dw", _sig(w))
         dx = torch.empty_like(x)
         dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
         if B * T == 0:
@@ -149,12 +156,14 @@ class Fused_RMS_Func(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x1, x2, w1, w2, norm_eps=1e-6, kernel_cache=None):
         x1, x2, w1, w2 = _lastdim_contig(x1, x2, w1, w2)
-        if not _seen(kernel_cache, "fwd", _sig(x1, x2, w1, w2)):
+        key = _sig(x1, x2, w1, w2)
+        if not _seen(kernel_cache, "fwd", key):
             _check_rows(x1)
             _check_rows(x2)
             assert x1.dtype == x2.dtype, "All tensors must have the same type"
             assert x1.shape[0] == x2.shape[0], f"{x1.shape=}, {x2.shape=}"
             assert w1.is_cuda and w2.is_cuda and w1.dtype in _FLOATS and w2.dtype in _FLOATS
+            _remember(kernel_cache, "fwd", key)
         l1, l2 = _w_layout(w1, x1), _w_layout(w2, x2)
         B, T1, C1 = x1.shape
         _, T2, C2 = x2.shape
@@ -177,8 +186,8 @@ class Fused_RMS_Func(torch.autograd.Function):
         (s1, sb1), (s2, sb2) = ctx.layouts
         B, T1, C1 = x1.shape
         _, T2, C2 = x2.shape
-        _seen(ctx.kernel_cache, "bwd", _sig(x1, x2, w1, w2, dy1, dy2))
-        _seen(ctx.kernel_cache, "bwd_dw", _sig(w1, w2))
+        _remember(ctx.kernel_cache, "bwd", _sig(x1, x2, w1, w2, dy1, dy2))
+        _remember(ctx.kernel_cache, "bwd_dw", _sig(w1, w2))
         dx1, dx2 = torch.empty_like(x1), torch.empty_like(x2)
         dw1 = torch.empty(w1.shape, dtype=w1.dtype, device=w1.device)
         dw2 = torch.empty(w2.shape, dtype=w2.dtype, device=w2.device)
@@ -210,8 +219,10 @@ class Norm_Func(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, norm_eps=1e-6, use_ptx=False, kernel_cache=None):
         (x,) = _lastdim_contig(x)
-        if not _seen(kernel_cache, "fwd", _sig(x)):
+        key = _sig(x)
+        if not _seen(kernel_cache, "fwd", key):
             _check_rows(x)
+            _remember(kernel_cache, "fwd", key)
         B, T, C = x.shape
         y = torch.empty_like(x)
         lib = _hip.lib()
@@ -228,7 +239,7 @@ class Norm_Func(torch.autograd.Function):
         (dy,) = _lastdim_contig(dy)
         (x,) = ctx.saved_tensors
         B, T, C = x.shape
-        _seen(ctx.kernel_cache, "bwd", _sig(x, dy))
+        _remember(ctx.kernel_cache, "bwd", _sig(x, dy))
         dx = torch.empty_like(x)
         lib = _hip.lib()
         _hip.check(lib.rgd_l2_bwd(B, T, C, t3(dy), t3(x), t3(dx), _hip.dtype_code(x.dtype), ctx.norm_eps,
@@ -246,11 +257,13 @@ class Fused_Norm_Func(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x1, x2, norm_eps=1e-6, kernel_cache=None):
         x1, x2 = _lastdim_contig(x1, x2)
-        if not _seen(kernel_cache, "fwd", _sig(x1, x2)):
+        key = _sig(x1, x2)
+        if not _seen(kernel_cache, "fwd", key):
             _check_rows(x1)
             _check_rows(x2)
             assert x1.dtype == x2.dtype, "All tensors must have the same type"
             assert x1.shape[0] == x2.shape[0], f"{x1.shape=}, {x2.shape=}"
+            _remember(kernel_cache, "fwd", key)
         B, T1, C1 = x1.shape
         _, T2, C2 = x2.shape
         y1, y2 = torch.empty_like(x1), torch.empty_like(x2)
@@ -269,7 +282,7 @@ class Fused_Norm_Func(torch.autograd.Function):
         x1, x2 = ctx.saved_tensors
         B, T1, C1 = x1.shape
         _, T2, C2 = x2.shape
-        _seen(ctx.kernel_cache, "bwd", _sig(x1, x2, dy1, dy2))
+        _remember(ctx.kernel_cache, "bwd", _sig(x1, x2, dy1, dy2))
         dx1, dx2 = torch.empty_like(x1), torch.empty_like(x2)
         lib = _hip.lib()
         _hip.check(lib.rgd_fused_l2_bwd(B, T1, C1, T2, C2, t3(dy1), t3(x1), t3(dx1), t3(dy2), t3(x2), t3(dx2),
@@ -335,8 +348,8 @@ class Fused_LNQK_Func(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, heads_second=True, norm_eps=1e-6, kernel_cache=None):
         q, k = _lastdim_contig(q, k)
-        _seen(kernel_cache, "fwd", _sig(q, k) + (heads_second,))
         B, H, Tq, Tk, D = _qk_dims(q, k, heads_second, 256, "head LayerNorm")
+        _remember(kernel_cache, "fwd", _sig(q, k) + (heads_second,))
         qo, ko = torch.empty_like(q), torch.empty_like(k)
         lib = _hip.lib()
         _hip.check(lib.rgd_ln_qk_fwd(B, H, Tq, Tk, D, t4(q, heads_second), t4(k, heads_second), t4(qo, heads_second),
@@ -355,7 +368,7 @@ class Fused_LNQK_Func(torch.autograd.Function):
         q, k = ctx.saved_tensors
         hs = ctx.heads_second
         doq, dok = _lastdim_contig(doq, dok)
-        _seen(ctx.kernel_cache, "bwd", _sig(q, k, doq, dok) + (hs,))
+        _remember(ctx.kernel_cache, "bwd", _sig(q, k, doq, dok) + (hs,))
         B, H, Tq, Tk, D = ctx.dims
         dq, dk = torch.empty_like(q), torch.empty_like(k)
         lib = _hip.lib()
@@ -375,9 +388,9 @@ class CombinedRoPEFunc(torch.autograd.Function):
         if in_place:
             assert q.stride(-1) == 1 and k.stride(-1) == 1, "in_place RoPE needs unit-stride head dims"
         q, k, pos_emb = _lastdim_contig(q, k, _table_for(pos_emb, q))
-        _seen(kernel_cache, "fwd", _sig(q, k, pos_emb) + (heads_second,))
         B, H, Tq, Tk, D = _qk_dims(q, k, heads_second, 128, "RoPE")
         pe = _pos_emb_args(pos_emb, Tq, Tk)
+        _remember(kernel_cache, "fwd", _sig(q, k, pos_emb) + (heads_second,))
         cq, ck = _cutoffs(seq_cutoff, Tq, Tk)
         if in_place:
             qo, ko = q, k
@@ -402,7 +415,7 @@ class CombinedRoPEFunc(torch.autograd.Function):
         assert not ctx.needs_input_grad[2], "CombinedRoPE does not support gradients in position embeddings"
         hs = ctx.heads_second
         doq, dok = _lastdim_contig(doq, dok)
-        _seen(ctx.kernel_cache, "bwd", _sig(doq, dok, pos_emb) + (hs,))
+        _remember(ctx.kernel_cache, "bwd", _sig(doq, dok, pos_emb) + (hs,))
         B, H, Tq, Tk, D = ctx.dims
         pe = _pos_emb_args(pos_emb, Tq, Tk)
         cq, ck = ctx.seq_cutoff
@@ -425,9 +438,9 @@ class FusedRoPEFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, pos_emb, seq_cutoff=None, heads_second=True, norm_eps=1e-6, kernel_cache=None):
         q, k, pos_emb = _lastdim_contig(q, k, _table_for(pos_emb, q))
-        _seen(kernel_cache, "fwd", _sig(q, k, pos_emb) + (heads_second,))
         B, H, Tq, Tk, D = _qk_dims(q, k, heads_second, 128, "LayerNorm+RoPE")
         pe = _pos_emb_args(pos_emb, Tq, Tk)
+        _remember(kernel_cache, "fwd", _sig(q, k, pos_emb) + (heads_second,))
         cq, ck = _cutoffs(seq_cutoff, Tq, Tk)
         qo, ko = torch.empty_like(q), torch.empty_like(k)
         lib = _hip.lib()
@@ -450,7 +463,7 @@ class FusedRoPEFunc(torch.autograd.Function):
         assert not ctx.needs_input_grad[2], "CombinedRoPE does not support gradients in position embeddings"
         hs = ctx.heads_second
         doq, dok = _lastdim_contig(doq, dok)
-        _seen(ctx.kernel_cache, "bwd", _sig(q, k, doq, dok, pos_emb) + (hs,))
+        _remember(ctx.kernel_cache, "bwd", _sig(q, k, doq, dok, pos_emb) + (hs,))
         B, H, Tq, Tk, D = ctx.dims
         pe = _pos_emb_args(pos_emb, Tq, Tk)
         cq, ck = ctx.seq_cutoff
@@ -536,13 +549,15 @@ def _bias_classes(bias, bdesc, bkind, bdtype, dims):
 def _flash_attn_forward(q, k, v, bias=None, causal=False, softmax_scale=None, kernel_cache=None, return_classes=False):
     batch, seqlen_q, nheads, d = q.shape
     _, seqlen_k, _, _ = k.shape
-    if not _seen(kernel_cache, "fwd", _sig(q, k, v, bias) + (bool(causal),)):
+    key = _sig(q, k, v, bias) + (bool(causal),)
+    if not _seen(kernel_cache, "fwd", key):
         assert k.shape == (batch, seqlen_k, nheads, d)
         assert v.shape == (batch, seqlen_k, nheads, d)
         assert d <= 128, "FlashAttention only support head dimensions up to 128"
         assert q.dtype == k.dtype == v.dtype, f"All tensors must have the same type {q.dtype=}, {k.dtype=}, {v.dtype=}"
         assert q.dtype in [torch.float16, torch.bfloat16], "Only support fp16 and bf16"
         assert q.is_cuda and k.is_cuda and v.is_cuda
+        _remember(kernel_cache, "fwd", key)
     softmax_scale = softmax_scale or 1.0 / math.sqrt(d)
     if bias is not None and bias.stride(-1) != 1:
         bias = bias.contiguous()
@@ -624,12 +639,14 @@ def _flash_attn_backward(do, q, k, v, o, lse, dq, dk, dv, bias=None, causal=Fals
     _, seqlen_k, _, _ = k.shape
     lib = _hip.lib()
     seqlen_q_rounded = lib.rgd_attn_seqlen_q_rounded(seqlen_q)
-    if not _seen(kernel_cache, "bwd", _sig(q, k, v, bias, do) + (bool(causal),)):
+    key = _sig(q, k, v, bias, do) + (bool(causal),)
+    if not _seen(kernel_cache, "bwd", key):
         assert d <= 128
         assert lse.shape == (batch, nheads, seqlen_q_rounded)
         assert q.stride(-1) == k.stride(-1) == v.stride(-1) == o.stride(-1) == 1
         assert dq.stride(-1) == dk.stride(-1) == dv.stride(-1) == 1
-    _seen(kernel_cache, "bwd_odot", _sig(o, do))
+        _remember(kernel_cache, "bwd", key)
+    _remember(kernel_cache, "bwd_odot", _sig(o, do))
     softmax_scale = softmax_scale or 1.0 / math.sqrt(d)
     if not bias_grad:
         _attn_bwd_call(do, q, k, v, o, lse, dq, dk, dv, bias, causal, softmax_scale, _bwd_mode(d), None, bias_classes)
@@ -777,11 +794,13 @@ def _bias_workspaces(nheads, seqlen_q, seqlen_k, num_buckets, code):
 def _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, kernel_cache):
     wstride = weight.stride()
     device = weight.device
-    if not _seen(kernel_cache, "fwd", kernel_cache and (weight.shape, wstride, weight.dtype, device, seqlen_q, seqlen_k, q_offset, dtype, ranges)):
+    key = kernel_cache and (weight.shape, wstride, weight.dtype, device, seqlen_q, seqlen_k, q_offset, dtype, ranges)
+    if not _seen(kernel_cache, "fwd", key):
         assert weight.is_cuda, "rgd_triton_amd operators run on the GPU only"
         assert weight.dtype in _FLOATS and dtype in _FLOATS, "Only support fp16, bf16, and fp32"
         assert weight.ndim == 2 and ranges.most < weight.shape[0], f"{weight.shape=}"
         assert seqlen_q >= 0 and seqlen_k >= 0, f"{seqlen_q=}, {seqlen_k=}"
+        _remember(kernel_cache, "fwd", key)
     index = device.index
     if index != _current_device():  # kernels are launched on the tensors' device, whichever is current
         with torch.cuda.device(index):
@@ -842,7 +861,7 @@ def _relative_bias_backward(ctx, dbias):
     num_buckets, nheads, wdtype = ctx.weight
     seqlen_q, seqlen_k, ranges, q_offset, _, kernel_cache = ctx.call
     if kernel_cache is not None:
-        _seen(kernel_cache, "bwd", _sig(dbias))
+        _remember(kernel_cache, "bwd", _sig(dbias))
     return _relative_bias_grad(dbias, num_buckets, nheads, seqlen_q, seqlen_k, ranges, q_offset, wdtype), None
 
 
@@ -924,8 +943,8 @@ def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_tabl
     shape, kshape, cshape = query.shape, key.shape, k_cache.shape
     index = query.get_device()
     dtype = query.dtype
-    if not _seen(kernel_cache, "fwd", kernel_cache and _sig(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens) +
-                 (bool(heads_second), index)):
+    sig = kernel_cache and _sig(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens) + (bool(heads_second), index)
+    if not _seen(kernel_cache, "fwd", sig):
         assert len(shape) == len(kshape) == 4
         assert dtype == key.dtype == value.dtype, "All tensors must have the same type"
         assert kshape == value.shape and kshape[0] == shape[0] and kshape[tok] == shape[tok] and kshape[3] == shape[3], \
@@ -940,6 +959,7 @@ def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_tabl
             assert pos_emb.shape[1] >= page_table.shape[1] * cshape[1], \
                 f"{pos_emb.shape=}: a row for every position of {page_table.shape[1]} pages of {cshape[1]}"
         _check_device(what, index, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens)
+        _remember(kernel_cache, "fwd", sig)
     if index != _current_device():
         with torch.cuda.device(index):
             return rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens, seq_cutoff,
@@ -1002,13 +1022,15 @@ def paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight
     shape, cache = q.shape, k_cache.shape
     index = q.get_device()
     dtype = q.dtype
-    if not _seen(kernel_cache, "fwd", kernel_cache and _sig(q, k_cache, v_cache, page_table, seq_lens, rel_weight) + (index,)):
+    sig = kernel_cache and _sig(q, k_cache, v_cache, page_table, seq_lens, rel_weight) + (index,)
+    if not _seen(kernel_cache, "fwd", sig):
         assert len(shape) == 4 and shape[1] == 1, f"{q.shape=}: one new token per sequence"
         _check_cache(what, k_cache, v_cache, page_table, seq_lens, shape[0], dtype, shape[3])
         assert cache[2] >= 1 and shape[2] % cache[2] == 0, f"{q.shape=}, {k_cache.shape=}: query heads in groups"
         if rel_weight is not None:
             assert rel_weight.ndim == 2 and rel_weight.shape[1] == shape[2] and rel_weight.dtype in _FLOATS, f"{rel_weight.shape=}"
         _check_device(what, index, k_cache, v_cache, page_table, seq_lens, rel_weight)
+        _remember(kernel_cache, "fwd", sig)
     if index != _current_device():
         with torch.cuda.device(index):
             return paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight, max_distance, bidirectional,
