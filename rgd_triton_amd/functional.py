@@ -72,7 +72,8 @@ def _no_capture(what):
 
 
 def _sig(*ts):
-    return tuple((tuple(t.shape), t.dtype, tuple(t.stride())) if t is not None else None for t in ts)
+    """What the checks of a call look at: its tensors' sizes, types, strides and the device of every one of them."""
+    return tuple((t.shape, t.dtype, t.stride(), t.get_device()) if t is not None else None for t in ts)
 
 
 # ----------------------------------------------------------------------------------------------
@@ -943,7 +944,7 @@ def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_tabl
     shape, kshape, cshape = query.shape, key.shape, k_cache.shape
     index = query.get_device()
     dtype = query.dtype
-    sig = kernel_cache and _sig(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens) + (bool(heads_second), index)
+    sig = kernel_cache and _sig(query, key, value, pos_emb, k_cache, v_cache, page_table, cache_lens, new_lens) + (bool(heads_second),)
     if not _seen(kernel_cache, "fwd", sig):
         assert len(shape) == len(kshape) == 4
         assert dtype == key.dtype == value.dtype, "All tensors must have the same type"
@@ -1022,7 +1023,7 @@ def paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight
     shape, cache = q.shape, k_cache.shape
     index = q.get_device()
     dtype = q.dtype
-    sig = kernel_cache and _sig(q, k_cache, v_cache, page_table, seq_lens, rel_weight) + (index,)
+    sig = kernel_cache and _sig(q, k_cache, v_cache, page_table, seq_lens, rel_weight)
     if not _seen(kernel_cache, "fwd", sig):
         assert len(shape) == 4 and shape[1] == 1, f"{q.shape=}: one new token per sequence"
         _check_cache(what, k_cache, v_cache, page_table, seq_lens, shape[0], dtype, shape[3])

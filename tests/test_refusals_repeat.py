@@ -14,16 +14,18 @@ BF, HF, FP, I32, I64 = torch.bfloat16, torch.float16, torch.float32, torch.int32
 
 
 class OnGpu(torch.Tensor):
-    """a CPU tensor that says it is on cuda:0"""
+    """a CPU tensor that says it is on a GPU, cuda:0 unless told otherwise"""
 
     is_cuda = True
 
     def get_device(self):
-        return 0
+        return self.__dict__.get("index", 0)
 
 
-def gpu(*shape, dtype=BF):
-    return torch.zeros(*shape, dtype=dtype).as_subclass(OnGpu)
+def gpu(*shape, dtype=BF, index=0):
+    t = torch.zeros(*shape, dtype=dtype).as_subclass(OnGpu)
+    t.index = index
+    return t
 
 
 @pytest.fixture
@@ -161,3 +163,34 @@ def test_bias_refused_again(launches, monkeypatch, weight, kw):
         assert not launches
         rgd.relative_position_bias_fn(gpu(32, 4), 5, 7, kernel_cache=cache)
         assert len(launches) == 1
+
+
+MOVED = [(i, name, where) for i, (_, good, _) in enumerate(EVERY) for name in good() for where in (("cpu", "cuda:1") if i < 3 else ("cpu",))]
+
+
+@pytest.mark.parametrize("i,name,where", MOVED, ids=[f"{NAMES[i]}: {name} on {where}" for i, name, where in MOVED])
+def test_each_tensor_on_another_device(launches, i, name, where):
+    """behind a good call of the same sizes: a tensor in host memory is refused by every operator, and by those that a serving loop calls
+    one on another GPU too"""
+    make, good, _ = EVERY[i]
+    with torch.no_grad():
+        m = _on_gpu(make())
+        m(**good())
+        assert len(launches) == 1
+        t = good()[name]
+        other = t.as_subclass(torch.Tensor) if where == "cpu" else gpu(*t.shape, dtype=t.dtype, index=1)
+        for _ in range(2):
+            with pytest.raises(AssertionError):
+                m(**{**good(), name: other})
+        assert len(launches) == 1
+
+
+def test_decode_bias_weight_on_another_device(launches):
+    m, good, w = rgd.PagedDecodeAttention(), _decode_args(), gpu(32, 4, dtype=FP)
+    rel = lambda w: types.SimpleNamespace(weight=w, max_distance=128, bidirectional=True)  # noqa: E731
+    with torch.no_grad():
+        m(**good, rel_bias=rel(w))
+        for other in (torch.zeros(32, 4), gpu(32, 4, dtype=FP, index=1)):
+            with pytest.raises(AssertionError):
+                m(**good, rel_bias=rel(other))
+    assert len(launches) == 1
