@@ -49,6 +49,9 @@ def _seen(cache, field, key):
     return plans is not None and key in plans
 
 
+_MOST_SIGNATURES = 1024  # of a cache field: with more (prompts of every length) it starts anew, a check costs microseconds
+
+
 def _remember(cache, field, key):
     """Keeps the signature of a call that has passed every check: a refused one has to be refused again."""
     if cache is None:
@@ -57,6 +60,8 @@ def _remember(cache, field, key):
     if plans is None:
         plans = set()
         setattr(cache, field, plans)
+    elif len(plans) >= _MOST_SIGNATURES:
+        plans.clear()
     plans.add(key)
 
 
@@ -795,12 +800,13 @@ def _bias_workspaces(nheads, seqlen_q, seqlen_k, num_buckets, code):
 def _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype, kernel_cache):
     wstride = weight.stride()
     device = weight.device
-    key = kernel_cache and (weight.shape, wstride, weight.dtype, device, seqlen_q, seqlen_k, q_offset, dtype, ranges)
+    # (lengths and offsets are not kept: a model that reads on in chunks has others with every call)
+    assert seqlen_q >= 0 and seqlen_k >= 0, f"{seqlen_q=}, {seqlen_k=}"
+    key = kernel_cache and (weight.shape, wstride, weight.dtype, device, dtype, ranges.most)
     if not _seen(kernel_cache, "fwd", key):
         assert weight.is_cuda, "rgd_triton_amd operators run on the GPU only"
         assert weight.dtype in _FLOATS and dtype in _FLOATS, "Only support fp16, bf16, and fp32"
         assert weight.ndim == 2 and ranges.most < weight.shape[0], f"{weight.shape=}"
-        assert seqlen_q >= 0 and seqlen_k >= 0, f"{seqlen_q=}, {seqlen_k=}"
         _remember(kernel_cache, "fwd", key)
     index = device.index
     if index != _current_device():  # kernels are launched on the tensors' device, whichever is current

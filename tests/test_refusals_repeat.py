@@ -1,5 +1,5 @@
 """A call that is refused stays refused: every Module keeps the signatures of the calls that passed its checks, so the same bad call
-is made twice, and once more behind a good one.  On the CPU: the library is a stand-in that records launches, the tensors say that
+is made twice, and once more behind a good one; and what it keeps does not grow for ever.  On the CPU: the library is a stand-in that records launches, the tensors say that
 they are on a GPU."""
 import types
 
@@ -194,3 +194,23 @@ def test_decode_bias_weight_on_another_device(launches):
             with pytest.raises(AssertionError):
                 m(**good, rel_bias=rel(other))
     assert len(launches) == 1
+
+
+def test_signatures_of_a_serving_loop_are_bounded(launches, monkeypatch):
+    """queries at other offsets and over other lengths, chunk after chunk, add nothing; prompts of every length stop at a bound"""
+    monkeypatch.setattr(F_, "_current_device", lambda: None)
+    cache = rgd.RelativePositionBias(32, 4).cache
+    w = gpu(32, 4)
+    with torch.no_grad():
+        for step in range(2 * F_._MOST_SIGNATURES):
+            rgd.relative_position_bias_fn(w, 0, step, q_offset=step, kernel_cache=cache)
+        assert len(cache.fwd) == 1
+        monkeypatch.setattr(F_, "_current_device", lambda: 0)
+        m = rgd.RoPECacheAppend()
+        for T in range(2 * F_._MOST_SIGNATURES + 7):
+            m(**{**_append_args(), **dict(query=gpu(2, 4, T, 64), key=gpu(2, 2, T, 64), value=gpu(2, 2, T, 64))})
+            assert len(m.cache.fwd) <= F_._MOST_SIGNATURES
+        assert len(m.cache.fwd) == 7
+        # still a check for whoever comes behind
+        with pytest.raises(AssertionError):
+            m(**{**_append_args(), **APPEND_BAD["int64 lengths"]})
