@@ -219,6 +219,7 @@ template <typename T> __global__ __launch_bounds__(256) void rel_bias_ordered_ke
 // part[(h * ranges + k) * tasks + task]: what the task adds to range k
 template <typename T> __global__ __launch_bounds__(256) void rel_bias_bwd_kernel(const RelParams p) {
     __shared__ double s_sum[4][STRIP + 8];
+    __shared__ alignas(8) uint8_t s_begin[4][STRIP + 8];  // a range begins at this diagonal
     const int h = blockIdx.y;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int task = blockIdx.x * 4 + wave;
@@ -282,41 +283,51 @@ template <typename T> __global__ __launch_bounds__(256) void rel_bias_bwd_kernel
             line[a] += lane > 0 ? left : 0.f;
         }
     }
-    // Ranges are differences of the diagonals' running sum, which is kept in 64 bits: a short range behind a long one loses
-    // nothing.
+    // A running sum of the diagonals, in 64 bits, that starts anew where a range begins: a range's sum is what stands at its last
+    // diagonal, and no range sees another's infinities or large numbers, as it would in differences of one running sum (those are
+    // 0.3 us shorter: (8, 128, 128) 7.0 / 7.3 us, (16, 2048, 2048) 28.4 / 28.8 us, (16, 1024, 1024) with 256 buckets 16.5 / 18.0 us).
     double* sum = s_sum[wave];
-    double total = line[0];
+    uint8_t* begin = s_begin[wave];
+    const int d0 = strip - i0 - 7 - p.offset;  // d of the first of STRIP + 7 diagonals
+    auto first_of = [&](int k) { return (int)min((int64_t)STRIP + 7, max((int64_t)0, (int64_t)p.r.start[k] - d0)); };
+    auto ordered = [] {  // (a wavefront's own LDS rows: its accesses are in order)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    reinterpret_cast<uint64_t*>(begin)[lane] = 0;
+    if (lane == 0) reinterpret_cast<uint64_t*>(begin)[64] = 0;
+    ordered();
+    for (int k = lane; k < p.r.n; k += 64)
+        if (k > 0) begin[first_of(k)] = 1;  // (range 0 has no beginning; STRIP + 7 is no diagonal)
+    ordered();
+    const uint64_t mine = reinterpret_cast<const uint64_t*>(begin)[lane], rest = reinterpret_cast<const uint64_t*>(begin)[64];
+    auto begins = [&](int a) { return ((a < 8 ? mine : rest) >> (8 * (a & 7)) & 1) != 0; };
+    double total = 0.;  // of the lane's diagonals from its last beginning on
 #pragma unroll
-    for (int a = 1; a < 8; ++a) total += line[a];
-    const double own = total;
+    for (int a = 0; a < 8; ++a) total = (begins(a) ? 0. : total) + line[a];
+    int any = mine != 0;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
         const double up = __shfl_up(total, m, 64);
-        if (lane >= m) total += up;
+        const int up_any = __shfl_up(any, m, 64);
+        if (lane >= m) {
+            total = any ? total : up + total;
+            any |= up_any;
+        }
     }
-    const bool finite = __all(isfinite(total));
-    double run = finite ? total - own : 0.;  // (an infinity or NaN stays in its own range: those sums are made one by one)
-    if (lane == 0) sum[0] = 0.;
+    const double before = __shfl_up(total, 1, 64);
+    double run = lane > 0 ? before : 0.;
 #pragma unroll
     for (int a = 0; a < 15; ++a) {
         if (a >= 8 && lane < 63) break;
-        const float v = a < 8 ? line[a & 7] : acc[a];
-        run = finite ? run + v : v;
-        sum[8 * lane + a + 1] = run;
+        run = (begins(a) ? 0. : run) + (a < 8 ? line[a & 7] : acc[a]);
+        sum[8 * lane + a] = run;
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (a wavefront's own LDS rows: its accesses are in order)
-    __builtin_amdgcn_wave_barrier();
-    const int d0 = strip - i0 - 7 - p.offset;  // d of the first of STRIP + 7 diagonals
+    ordered();
     float* out = static_cast<float*>(p.part) + (int64_t)h * p.r.n * p.tasks + task;
     for (int k = lane; k < p.r.n; k += 64) {
-        const int lo = k == 0 ? 0 : (int)min((int64_t)STRIP + 7, max((int64_t)0, (int64_t)p.r.start[k] - d0));
-        const int hi = k + 1 < p.r.n ? (int)min((int64_t)STRIP + 7, max((int64_t)0, (int64_t)p.r.start[k + 1] - d0)) : STRIP + 7;
-        double s = sum[hi] - sum[lo];
-        if (!finite) {
-            s = 0.;
-            for (int e = lo; e < hi; ++e) s += sum[e + 1];
-        }
-        out[(int64_t)k * p.tasks] = (float)s;
+        const int lo = k == 0 ? 0 : first_of(k), hi = k + 1 < p.r.n ? first_of(k + 1) : STRIP + 7;
+        out[(int64_t)k * p.tasks] = hi > lo ? (float)sum[hi - 1] : 0.f;
     }
 }
 
