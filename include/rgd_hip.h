@@ -348,7 +348,8 @@ int rgd_rope_cache_append(const rgd_cache_append_args* args, void* stream);
  * receives log sum_j exp of the logits.  A sequence without keys, or with no logit above -inf, gives o = 0 and lse = -inf.
  * rel_weight (NULL: no bias): bias_j = weight[bucket * w_stride + h] of the range (see rgd_rel_bias_fwd) that holds
  * j - (seq_lens[b] - 1); starts and buckets are HOST arrays, read during the call.
- * Statistics and sums are fp32; every result is reproducible bit for bit.  Calls that may overlap in time need separate
+ * Statistics and sums are fp32; every result is reproducible bit for bit.  In fp16 a probability is held to 2^-33 of the largest: an
+ * infinite value under one below 2^-25 may come out as NaN.  Calls that may overlap in time need separate
  * workspaces (any contents on entry, 16-byte aligned).  B * Hq below 2^24. */
 size_t rgd_paged_decode_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
 typedef struct rgd_paged_decode_args {

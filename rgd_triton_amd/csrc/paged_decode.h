@@ -23,7 +23,8 @@
 // So 16 rows of heads are computed whatever the group: at the rate the memory delivers keys the matrix pipe is busy a tenth of
 // the time.  P is split into two 16-bit parts (a second product each): rounded to one, its error would be as large as the
 // output's own rounding, and the products are free (DEC_HIGH).
-// The running maximum is a reference that moves only when a logit exceeds it by LAZY; sums, maxima and outputs are fp32.
+// The running maximum is a reference that moves only when a logit exceeds it by LAZY (fp16: it stays a headroom below the
+// maximum); sums, maxima and outputs are fp32.
 //
 // Measured (this launch / the merge; a read that streams 512 MB reaches 6.6 TB/s): one sequence of 131000 keys, 32 / 8 heads,
 // D = 128: 86 / 7 us, 6.2 TB/s; 64 sequences to 4100 keys, the same heads: 106 / 5 us, 5.5 TB/s; 19 to 2000 keys, 24 heads,
@@ -108,13 +109,18 @@ __device__ __forceinline__ float xor_lanes(float v, int m) { return __shfl_xor(v
 // one sequence of 131000 keys took 100 us instead of 95.
 #define DEC_KEEP_LOADS() __builtin_amdgcn_sched_barrier(0)
 
-// log2(e) and how far a logit may exceed the reference before that moves: probabilities stay below e^5.5 = 245
+// log2(e) and how far a logit may exceed the reference and its headroom before that moves: probabilities stay below
+// e^(5.5 + headroom)
 constexpr float DEC_LOG2E = 1.4426950408889634f;
 constexpr float DEC_LAZY = 5.5f;
+// The reference is the running maximum less a headroom.  fp16 ends at 65504 above and at 2^-24 below: with 2^8 of headroom (e^5.5
+// 2^8 = 62600) a key counts down to 2^-33 of the largest instead of 2^-25 (32768 equal keys 2^-25 below one other, which are 0.1 %
+// of the sum, would add nothing to the output).  bf16 ends where fp32 does.
+template <typename T> constexpr float DEC_HEADROOM = std::is_same<T, f16_t>::value ? 8.0f * 0.6931471805599453f : 0.0f;
 // The high part of a probability is the 16-bit rounding of (1 - 2^-7) p, the low part the rounding of what is left: below p
-// by more than half a step of the type (bf16: 2^-8), so the low part is positive wherever p is (down to 2^-18 in fp16, whose
-// subnormal numbers end the split), and an infinite value stays infinite instead of meeting a zero or a negative factor.
-// What is left is at most (2^-7 + 2^-8) p, its own rounding 2^-14.4 p.
+// by more than half a step of the type (bf16: 2^-8), so the low part is positive wherever p is (in fp16 down to 2^-25 of the
+// largest, below which its subnormal numbers end the split), and an infinite value stays infinite instead of meeting a zero or a
+// negative factor.  What is left is at most (2^-7 + 2^-8) p, its own rounding 2^-14.4 p (fp16: or 2^-33 of the largest).
 constexpr float DEC_HIGH = 1.0f - 1.0f / 128;
 
 // NC: 32-channel chunks of the head dim (DP = 32 NC).  SMALL: D < 8, rows are read element by element.  LINES: D = DP is 64 or 128,
@@ -448,10 +454,11 @@ __global__ __launch_bounds__(64, 2) void paged_decode_kernel(const DecodeParams 
                     if (!(t + 8 * g + i < len && (ok8 >> i & 1))) x8[i] = -INFINITY;
             }
             float top = fmaxf(fmaxf(fmaxf(x8[0], x8[1]), fmaxf(x8[2], x8[3])), fmaxf(fmaxf(x8[4], x8[5]), fmaxf(x8[6], x8[7])));
-            if (__any(top > ref + DEC_LAZY)) {
+            // (the difference, not a sum: of large logits a sum may round up past what fp16 holds)
+            if (__any(top - ref > DEC_LAZY + DEC_HEADROOM<T>)) {
                 top = fmaxf(top, xor_lanes(top, 16));
                 top = fmaxf(top, xor_lanes(top, 32));
-                const float moved = fmaxf(ref, top);
+                const float moved = fmaxf(ref, top - DEC_HEADROOM<T>);
                 // (a head that has seen no logit yet has nothing to rescale)
                 const float f = ref == -INFINITY ? 0.f : exp2f((ref - moved) * DEC_LOG2E);
                 l *= f;
