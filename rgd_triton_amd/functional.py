@@ -24,6 +24,7 @@ import math
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _hip
 from ._hip import t3, t4
@@ -74,6 +75,13 @@ def _no_capture(what):
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{what}: an autograd backward cannot be recorded into a HIP graph with this package; "
                            "record direct calls of the C ABI instead")
+
+
+def _no_tangent(what, *ts):
+    """For what goes round autograd: a forward-mode derivative is refused, as autograd functions without one refuse it."""
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            assert t is None or forward_ad.unpack_dual(t).tangent is None, f"{what} has no forward-mode derivative"
 
 
 def _sig(*ts):
@@ -884,6 +892,7 @@ def relative_position_bias_fn(weight, seqlen_q, seqlen_k, max_distance=128, bidi
     if weight.stride(-1) != 1:
         weight = weight.contiguous()
     ranges = relative_ranges(weight.shape[0], max_distance, bool(bidirectional))
+    _no_tangent("relative_position_bias", weight)
     if torch.is_grad_enabled() and weight.requires_grad:
         return Relative_Bias_Func.apply(weight, (seqlen_q, seqlen_k, ranges, q_offset, dtype or weight.dtype, kernel_cache))
     return _relative_bias(weight, seqlen_q, seqlen_k, ranges, q_offset, dtype or weight.dtype, kernel_cache)
@@ -946,6 +955,7 @@ def rope_cache_append_fn(query, key, value, pos_emb, k_cache, v_cache, page_tabl
         (pos_emb,) = _lastdim_contig(_table_for(pos_emb, query))
     if torch.is_grad_enabled():
         _no_grad(what, query, key, value, pos_emb, k_cache, v_cache)
+    _no_tangent(what, query, key, value, pos_emb, k_cache, v_cache)
     head, tok = (1, 2) if heads_second else (2, 1)
     shape, kshape, cshape = query.shape, key.shape, k_cache.shape
     index = query.get_device()
@@ -1026,6 +1036,7 @@ def paged_decode_attn_func(q, k_cache, v_cache, page_table, seq_lens, rel_weight
         rel_weight = rel_weight.contiguous()
     if torch.is_grad_enabled():
         _no_grad(what, q, k_cache, v_cache, rel_weight)
+    _no_tangent(what, q, k_cache, v_cache, rel_weight)
     shape, cache = q.shape, k_cache.shape
     index = q.get_device()
     dtype = q.dtype

@@ -214,3 +214,49 @@ def test_signatures_of_a_serving_loop_are_bounded(launches, monkeypatch):
         # still a check for whoever comes behind
         with pytest.raises(AssertionError):
             m(**{**_append_args(), **APPEND_BAD["int64 lengths"]})
+
+
+# ------------------------------------------------------------------ derivatives that are not there
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(launches, monkeypatch, grad):
+    """a tensor that carries a tangent would give a result without one; outside of its level, and beside other levels, calls go on"""
+    from torch.autograd import forward_ad
+
+    def dual(t):
+        return forward_ad.make_dual(t, torch.ones_like(t))
+
+    monkeypatch.setattr(F_, "_current_device", lambda: None)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        w = gpu(32, 4, dtype=FP)
+        with pytest.raises(AssertionError, match="forward-mode"):
+            rgd.relative_position_bias_fn(dual(w), 5, 7)
+        rgd.relative_position_bias_fn(w, 5, 7)
+        monkeypatch.setattr(F_, "_current_device", lambda: 0)
+        for name in ("query", "key", "value", "pos_emb", "k_cache", "v_cache"):
+            args = _append_args()
+            with pytest.raises(AssertionError, match="forward-mode"):
+                rgd.RoPECacheAppend()(**{**args, name: dual(args[name])})
+        for name in ("q", "k_cache", "v_cache"):
+            args = _decode_args()
+            with pytest.raises(AssertionError, match="forward-mode"):
+                rgd.PagedDecodeAttention()(**{**args, name: dual(args[name])})
+        with pytest.raises(AssertionError, match="forward-mode"):
+            rgd.paged_decode_attn_func(**_decode_args(), rel_weight=dual(w))
+    assert launches == ["rgd_rel_bias_fwd"]
+    with torch.no_grad():
+        rgd.PagedDecodeAttention()(**_decode_args())
+    assert len(launches) == 2
+
+
+def test_functional_derivatives_are_refused(launches, monkeypatch):
+    """torch.func's transforms hand in wrappers without memory of their own"""
+    monkeypatch.setattr(F_, "_current_device", lambda: None)
+    f = lambda w: rgd.relative_position_bias_fn(w, 5, 7)  # noqa: E731
+    w = torch.zeros(32, 4)
+    for transform in (lambda: torch.func.jvp(f, (w,), (torch.ones_like(w),)), lambda: torch.func.grad(lambda x: f(x).sum())(w),
+                      lambda: torch.func.vmap(f)(torch.zeros(3, 32, 4))):
+        with pytest.raises((AssertionError, RuntimeError)):
+            transform()
+    assert not launches
