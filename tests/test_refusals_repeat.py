@@ -198,6 +198,7 @@ def test_decode_bias_weight_on_another_device(launches):
 
 def test_signatures_of_a_serving_loop_are_bounded(launches, monkeypatch):
     """queries at other offsets and over other lengths, chunk after chunk, add nothing; prompts of every length stop at a bound"""
+    monkeypatch.setattr(F_, "_MOST_SIGNATURES", 64)
     monkeypatch.setattr(F_, "_current_device", lambda: None)
     cache = rgd.RelativePositionBias(32, 4).cache
     w = gpu(32, 4)
