@@ -42,7 +42,7 @@ enum rgd_status {
     RGD_ERR_INVALID = -1,     /* bad argument (shape, dtype code, null pointer)          */
     RGD_ERR_UNSUPPORTED = -2, /* valid but outside what the kernels cover                 */
     RGD_ERR_LAUNCH = -3,      /* hipLaunchKernel reported an error                        */
-    RGD_ERR_WORKSPACE = -4    /* caller-provided workspace too small                      */
+    RGD_ERR_WORKSPACE = -4    /* caller-provided workspace too small or misaligned        */
 };
 
 enum rgd_bias_kind { RGD_BIAS_NONE = 0, RGD_BIAS_VECTOR = 1, RGD_BIAS_MATRIX = 2 };

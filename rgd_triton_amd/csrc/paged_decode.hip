@@ -123,6 +123,7 @@ int rgd_paged_decode(const rgd_paged_decode_args* args, void* stream) {
     hipStream_t s = static_cast<hipStream_t>(stream);
     RGD_REQUIRE(workspace && workspace_bytes >= rgd_paged_decode_workspace(B, Hq, Hkv, D), RGD_ERR_WORKSPACE,
                 "%s: workspace of %zu bytes, needs %zu", name, workspace_bytes, rgd_paged_decode_workspace(B, Hq, Hkv, D));
+    RGD_REQUIRE(rgd_aligned16(workspace), RGD_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", name);
     p.plan = static_cast<int*>(workspace);
     p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (B * Hkv * p.head_tiles * 2 * (int64_t)sizeof(int) + 15) / 16 * 16);
     if (none) {

@@ -444,6 +444,7 @@ int rgd_rel_bias_fwd(int64_t H, int64_t Tq, int64_t Tk, const void* weight, int6
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (workspace && workspace_bytes > 0 && workspace_bytes >= rgd_rel_bias_fwd_workspace(H, Tq, Tk, bias_dtype) &&
         rgd_rel_bias_fwd_workspace(H, Tq, Tk, bias_dtype) > 0) {
+        RGD_REQUIRE(rgd_aligned16(workspace), RGD_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", name);
         p.part = workspace;
         p.width = (int)values_of(Tq, Tk);
         return bias_dtype == RGD_F16 ? ordered<f16_t>(name, p, s) : bias_dtype == RGD_BF16 ? ordered<bf16_t>(name, p, s) : ordered<float>(name, p, s);
@@ -472,6 +473,7 @@ int rgd_rel_bias_bwd(int64_t H, int64_t Tq, int64_t Tk, const rgd_tensor4* dbias
     RGD_REQUIRE(dweight && (empty || (dbias && dbias->ptr)), RGD_ERR_INVALID, "%s: null tensor", name);
     RGD_REQUIRE(workspace_bytes >= rgd_rel_bias_bwd_workspace(H, Tq, Tk, num_buckets) && (empty || workspace), RGD_ERR_WORKSPACE,
                 "%s: workspace of %zu bytes, needs %zu", name, workspace_bytes, rgd_rel_bias_bwd_workspace(H, Tq, Tk, num_buckets));
+    RGD_REQUIRE(empty || rgd_aligned16(workspace), RGD_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", name);
     RelParams p;
     fill(&p, H, Tq, Tk, n_ranges, starts, buckets, q_offset, dbias);
     p.part = static_cast<float*>(workspace);
