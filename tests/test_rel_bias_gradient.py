@@ -1,9 +1,10 @@
-"""The gradient of the learned relative position bias's weight: infinities, NaN and large numbers stay in their bucket, wherever in a
-strip of diagonals they stand."""
+"""The gradient of the learned relative position bias's weight: every pair counted once, whatever the sizes and strides; the rounding of a
+32-bit sum no larger than its longest chain; infinities, NaN and large numbers in their own bucket, wherever in a strip of
+diagonals they stand."""
 import pytest
 import torch
 
-from serving_helpers import gen, serving_oracle
+from serving_helpers import dev, gen, half_step, randn, serving_oracle, spread
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +68,50 @@ def test_many_ranges_in_a_strip():
         dy = torch.randint(-4, 5, (1, 3, Tq, Tk), generator=gen(602)).float()
         want, _ = serving_oracle.relative_bias_grad(dy, 256, 900, both, off)
         assert torch.equal(_grad(dy.cuda(), 256, 900, both, off).cpu().double(), want)
+
+
+SHAPES = [(1, 1, 0), (1, 700, 699), (700, 1, 0), (7, 5, 0), (64, 64, 0), (129, 257, 128), (255, 1031, -40), (530, 520, 0), (1025, 300, 5000), (520, 1100, 3),
+          (2, 4099, 2048), (33, 2049, 0), (600, 7, -300), (16, 512, 0), (17, 505, 1)]
+BUCKETS = [(32, 128, True), (32, 128, False), (8, 20, True), (64, 700, True), (2, 5, False), (5, 9, False), (256, 900, True)]
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("Tq,Tk,off", SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("wdtype", DTYPES)
+def test_whole_numbers_are_exact(Tq, Tk, off, dtype, wdtype):
+    """sums of whole numbers up to 4 stay below 2^24: exact in 32 bits, rounded once to the weight's type.  A pair left out or counted
+    twice shows, in every layout"""
+    i = SHAPES.index((Tq, Tk, off))
+    nb, md, both = BUCKETS[(i + DTYPES.index(dtype)) % len(BUCKETS)]
+    H = 1 + i % 4
+    dy = torch.randint(1, 5, (1, H, Tq, Tk), generator=gen(640 + i)).to(dtype)
+    layouts = {"plain": dev(dy), "gaps": dev(spread(dy, (2, 3))), "shifted": dev(torch.cat([dy[..., :1], dy], -1))[..., 1:],
+               "heads inside": dev(dy.transpose(1, 2).contiguous()).transpose(1, 2)}
+    # the values up to 4 x 307500 pairs: fp16 ends at 65504, where the rounding is to infinity
+    want = serving_oracle.relative_bias_grad(dy, nb, md, both, off)[0].float().to(wdtype)
+    for name, x in layouts.items():
+        got = _grad(x, nb, md, both, off, wdtype).cpu()
+        assert torch.equal(got, want), (name, (got.double() - want.double()).abs().max())
+
+
+@pytest.mark.parametrize("Tq,Tk,off", SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rounding_of_the_sums(Tq, Tk, off, dtype):
+    """The chain of 32-bit additions: at most `chunk` rows of a diagonal in a lane's register, one neighbour's, one rounding of the 64-bit
+    sum; then a lane's share of the tasks (every 256th in each of four sums, the rest in one), two joins of the four and six of
+    the lanes; one rounding.  chunk is the longest of 256 .. 16 that leaves 8 wavefronts to a compute unit."""
+    i = SHAPES.index((Tq, Tk, off))
+    nb, md, both = BUCKETS[(i + 3 * DTYPES.index(dtype)) % len(BUCKETS)]
+    H = 1 + i % 4
+    dy = randn(gen(660 + i), 1, H, Tq, Tk, dtype=dtype, shift=0.3)
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    for chunk in (256, 128, 64, 32, 16):
+        tasks = -(-Tq // chunk) * -(-(Tk + chunk - 8) // 512)
+        if tasks * H >= 8 * cus:
+            break
+    depth = chunk + 2 + tasks // 256 + 4 + 8
+    ref, mag = serving_oracle.relative_bias_grad(dy, nb, md, both, off)
+    got = _grad(dev(dy), nb, md, both, off).cpu().double()
+    tol = depth * 2.0**-24 * mag
+    assert ((got - ref).abs() <= tol + half_step(torch.float32) * (ref.abs() + tol)).all(), ((got - ref).abs() / tol.clamp(min=1e-30)).max()
