@@ -1,5 +1,5 @@
-"""PagedDecodeAttention far below the largest probability: keys that weigh next to nothing each and something together, infinite
-values under small weights, logits so large that neighbouring numbers are far apart."""
+"""PagedDecodeAttention at the ends of its ranges: keys that weigh next to nothing each and something together, infinite values under
+small weights, logits so large that neighbouring numbers are far apart, thousands of sequences."""
 import math
 
 import pytest
@@ -105,3 +105,32 @@ def test_logits_so_large_that_steps_are_whole(top, dtype):
     bound = (2.0**-17 + 2.0**-13 + 112 * 2.0**-23) * mag
     assert ((o[0, 0].double().cpu() - ref).abs() <= half_step(dtype) * (ref.abs() + bound) + bound).all()
     assert ((lse[0].double().cpu() - torch.logsumexp(s, -1)).abs() <= 2.0**-23 * top + 2.0**-18).all()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,size,most,dtype", [(2, 1, 64, 4, 9, BF), (3, 3, 40, 16, 70, HF)])
+def test_thousands_of_sequences(Hq, Hkv, D, size, most, dtype):
+    """6000 sequences, a third of them empty: a wavefront finds its run behind 94 looks at the lengths.  Checked on the GPU in 64 bits"""
+    from rgd_triton_amd import paged_decode_attn_func
+
+    B, g = 6000, gen(640)
+    each = -(-most // size)
+    pages = torch.randperm(B * each, generator=g).to(torch.int32).reshape(B, each).cuda()
+    lens = torch.randint(0, most + 1, (B,), generator=g, dtype=torch.int32)
+    lens[::3] = 0
+    lens = lens.cuda()
+    q = randn(g, B, 1, Hq, D, dtype=dtype).cuda()
+    k, v = (randn(g, B * each, size, Hkv, D, dtype=dtype, shift=0.2).cuda() for _ in range(2))
+    o, lse = paged_decode_attn_func(q, k, v, pages, lens, return_lse=True)
+    kk, vv = (c[pages.long()].reshape(B, each * size, Hkv, D).double().repeat_interleave(Hq // Hkv, 2) for c in (k, v))
+    s = (kk * q.double()).sum(-1) * D**-0.5  # (B, keys, Hq)
+    reach = ((kk * q.double()).abs().sum(-1) * D**-0.5).max().item()
+    s = s.masked_fill((torch.arange(each * size, device="cuda") >= lens[:, None])[..., None], -math.inf)
+    p = torch.softmax(s, 1).nan_to_num(0.0)
+    ref, mag = ((p[..., None] * x).sum(1)[:, None] for x in (vv, vv.abs()))
+    # as check_decode has it: products and sums of a logit, the exponential, the parts of a probability, sums over the keys
+    bound = (2 * ((D + 4) * 2.0**-24 * reach + 2.0**-22 * (reach + 10)) + 2 * (most + 16) * 2.0**-24 + 2.0**-14) * mag
+    assert ((o.double() - ref).abs() <= half_step(dtype) * (ref.abs() + bound) + bound + 2.0**-25).all()
+    rlse = torch.logsumexp(s, 1)
+    assert torch.equal(lse[lens == 0], torch.full_like(lse[lens == 0], -math.inf)) and torch.isfinite(lse[lens > 0]).all()
+    seen = lens > 0
+    assert ((lse[seen].double() - rlse[seen]).abs() <= (D + 4) * 2.0**-24 * reach + 2.0**-21 * (reach + 10)).all()
