@@ -6,8 +6,9 @@
 namespace {
 
 int chunks_of(int64_t D) { return (int)((D + 31) / 32); }
-// Wavefronts of the decode launch: those that are resident at once by their registers, three per SIMD for head dims up to 64, two
-// above.  More wait for their turn and leave more pieces to join, fewer leave loads in flight unused: at 1 / 2 / 3 per SIMD
+// Wavefronts of the decode launch, three per SIMD for head dims up to 64, two above: what the registers of most variants let be
+// resident at once (D up to 32, 128 registers, would let four; D = 33 .. 63 with bias, 169, lets two, and a third of the runs waits).
+// More wait for their turn and leave more pieces to join, fewer leave loads in flight unused: at 1 / 2 / 3 per SIMD
 // (D = 64, 24 heads, 19 lengths to 2000) 44 / 35 / 33 us, (D = 128, 8 key heads, 64 lengths to 4100) 112 / 113 / 117 us,
 // (D = 128, 24 heads, 19 lengths to 2000) 58 / 54 / 57 us.
 int64_t decode_grid(int64_t D) { return (int64_t)rgd_num_cus() * 4 * (D <= 64 ? 3 : 2); }

@@ -16,7 +16,8 @@
 // side in the order they are launched, and 4 from the walk, whose workgroups write 8 rows each all over the matrix.  The
 // values of a head's diagonals are first laid out in a row of the workspace (read back from the L2), then each thread takes
 // 8 columns of two rows (one row: too few bytes in flight for a round trip to the L2, 4.4 TB/s; four rows 5.7, two 6.2).
-// bf16, walk / address order: (24, 4352, 4352) 222 / 172 us, (16, 2048, 2048) 33 / 26 us, (16, 1024, 1024) 10.5 / 11 us.
+// bf16, walk / address order: (24, 4352, 4352) 222 / 172 us, (16, 2048, 2048) 33 / 26 us, (16, 1024, 1024) 10.5 / 11 us.  (Between
+// 34 and 134 MB, and in fp32, where the walk reaches 3.2 TB/s at 50 MB, the border was not looked for.)
 // Rows need no alignment: those written in address order are cut at the 16-byte boundaries of each row, the walk loads and stores
 // at any address, which the hardware takes.  A block that the last column cuts is read further left and shifted (element
 // by element its wavefront was the last to end: (24, 4352, 4351) bf16 381 us instead of 165).
