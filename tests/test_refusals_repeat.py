@@ -251,6 +251,21 @@ def test_forward_mode_derivatives_are_refused(launches, monkeypatch, grad):
     assert len(launches) == 2
 
 
+@pytest.mark.gpu
+def test_host_memory_behind_a_good_call_on_the_gpu():
+    """the same with real tensors: nothing is launched on lengths or tables in host memory"""
+    on = lambda args: {n: t.as_subclass(torch.Tensor).cuda() for n, t in args.items()}  # noqa: E731
+    with torch.no_grad():
+        for m, good, names in ((rgd.RoPECacheAppend(), on(_append_args()), ("page_table", "cache_lens", "new_lens", "pos_emb")),
+                               (rgd.PagedDecodeAttention(), on(_decode_args()), ("page_table", "seq_lens", "v_cache"))):
+            out = m(**good)
+            for name in names:
+                for _ in range(2):
+                    with pytest.raises(AssertionError):
+                        m(**{**good, name: good[name].cpu()})
+            assert torch.equal(m(**good), out)
+
+
 def test_functional_derivatives_are_refused(launches, monkeypatch):
     """torch.func's transforms hand in wrappers without memory of their own"""
     monkeypatch.setattr(F_, "_current_device", lambda: None)
