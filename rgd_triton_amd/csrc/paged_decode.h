@@ -28,7 +28,7 @@
 //
 // Measured (this launch / the merge; a read that streams 512 MB reaches 6.6 TB/s): one sequence of 131000 keys, 32 / 8 heads,
 // D = 128: 86 / 7 us, 6.2 TB/s; 64 sequences to 4100 keys, the same heads: 106 / 5 us, 5.5 TB/s; 19 to 2000 keys, 24 heads,
-// D = 80, bias, pages of 5: 40 / 5 us; one of 200 keys, 16 heads, D = 64: 5.3 / 3.6 us.  What a launch takes beyond its
+// D = 80, bias, pages of 5: 40 / 5 us; one of 200 keys, 16 heads, D = 64: 5.4 / 3.9 us.  What a launch takes beyond its
 // bytes, about 15 us, is the chain of loads in front of the first step (lengths, page numbers, keys), the last steps, in which
 // the wavefronts run out one by one, and the merge.
 #pragma once
